@@ -54,6 +54,7 @@ extern "C" {
 #define ATTN_ERR_TIMEOUT       -7  /* a bounded on-device wait expired             */
 #define ATTN_ERR_UNSUPPORTED   -8  /* valid op, variant not built (e.g. head_dim)  */
 #define ATTN_ERR_NO_DEVICE     -9  /* no sm_100 device visible                     */
+#define ATTN_ERR_CAPACITY     -10  /* a page pool, table or slot list is too small */
 
 /* ---- element types and mask kinds --------------------------------------- */
 #define ATTN_F32   0
@@ -277,6 +278,163 @@ ATTN_API int32_t _mlir_ciface_attn_fused_e4m3_causal_4d(AttnMemRef4D* Q, AttnMem
  * the caller.  Calls no cudaMalloc, cudaFree or allocating library routine. */
 #define ATTN_NOALLOC_SCRATCH_BYTES (64u << 20)
 ATTN_API int attn_fwd_host_noalloc(const AttnDesc* desc, void* stream);
+
+/* ---- paged key/value cache and the attention that reads it -----------------
+ * No counterpart in the reference, whose op takes whole Q, K and V.  These
+ * serve a model token by token: K and V of the tokens seen so far live in
+ * pages of `page_size` tokens (a power of two, 16 to 1024), a page being one
+ * [Hkv, page_size, D] slice of k_cache / v_cache [num_pages, Hkv, page_size, D].
+ * block_table[b] lists the pages of request b in order; token i of the request
+ * sits at slot block_table[b][i / page_size] * page_size + i % page_size.
+ *
+ * A step of a served batch: attn_cache_plan grows and shrinks the requests'
+ * page lists and gives each new token its position and slot; attn_rotary turns
+ * Q and K by those positions; attn_tree_fwd attends from the new tokens over
+ * the cached ones and over each other; attn_cache_append writes the accepted
+ * tokens' K and V to their slots.
+ *
+ * All calls are asynchronous on `stream` and take device pointers.  Lengths,
+ * tables and slots are device data that the host never sees: what is wrong with
+ * them is recorded in the status word (`status`, or the runtime's per-device
+ * word when null; attn_rt_check_status) and the rows concerned are skipped.
+ * Calls may be captured into CUDA graphs and run on several streams at once,
+ * as long as the buffers they write differ. */
+#define ATTN_FLAG_DEVICE_POINTERS 1 /* flags: the caller vouches that every data
+                                       pointer is device memory (not looked up)  */
+
+/* Grow or shrink every request to targets[b] tokens.  p(n) = ceil(n / page_size).
+ * Pages that shrinking requests give back are pushed on the stack free_pages
+ * [num_pages] (request by request, in page order), then growing requests take
+ * their pages from its top in the same order: free_count counts the stack.
+ *   starts[b]     new tokens of the requests before b; starts[B] is their total
+ *   positions[i]  position of new token i in its request    (0 past the total)
+ *   slots[i]      its slot in the cache                     (-1 past the total)
+ *   lengths_out   targets; may be `lengths` (in place)
+ *   free_count_out  what the stack then holds; may be `free_count`
+ * Entries of block_table past a request's pages, and of free_pages past its
+ * count, are left as they were.  All or nothing: where the pages, the table's
+ * width or `tokens` do not suffice (ATTN_ERR_CAPACITY) or a length is out of
+ * range (ATTN_ERR_INVALID), nothing is allocated or released, lengths_out and
+ * free_count_out repeat their inputs, starts are 0 and slots -1. */
+typedef struct AttnCachePlan {
+  int32_t flags;
+  int32_t page_size;
+  int64_t B, W;            /* requests (<= 8192), columns of block_table          */
+  int64_t num_pages;       /* elements of free_pages                              */
+  int64_t tokens;          /* elements of slots and positions                     */
+  int64_t table_stride;    /* elements between rows of block_table                */
+  const int32_t* lengths;  /* [B] tokens held                                     */
+  const int32_t* targets;  /* [B] tokens wanted                                   */
+  int32_t* block_table;    /* [B, W]                                              */
+  int32_t* free_pages;     /* [num_pages]                                         */
+  const int32_t* free_count;
+  int32_t* lengths_out;
+  int32_t* free_count_out;
+  int32_t* starts;         /* [B + 1]                                             */
+  int32_t* positions;      /* [tokens], or null                                   */
+  int64_t* slots;          /* [tokens]                                            */
+  int32_t* status;
+} AttnCachePlan;
+ATTN_API int attn_cache_plan(const AttnCachePlan* desc, void* stream);
+
+/* Write K and V rows into the cache: row rows[i] (i when rows is null) goes to
+ * slot slots[i]; slots of -1 are passed over, so a padded batch or a drafted
+ * tree's rejected tokens need no packing.  bf16 / f16 rows go into a cache of
+ * their type, or into an e4m3 cache divided by the descale and saturated to
+ * +-448 (a NaN stays NaN).  Slots other than -1 must differ: of two rows sent
+ * to one slot either may stay, also in part.  A slot or row out of range is
+ * skipped and recorded (ATTN_ERR_INVALID).  Strides in elements, head_dim
+ * unit-stride and a multiple of 16; rows start on 16-byte boundaries. */
+typedef struct AttnCacheAppend {
+  int32_t flags;
+  int32_t dtype;           /* of k and v: ATTN_BF16 or ATTN_F16                   */
+  int32_t cache_dtype;     /* the same, or ATTN_E4M3                              */
+  int32_t page_size;
+  int64_t N, T;            /* slots; rows of k and v                              */
+  int64_t Hkv, D, num_pages;
+  int64_t k_stride[2], v_stride[2];               /* token, head                  */
+  int64_t k_cache_stride[3], v_cache_stride[3];   /* page, head, token            */
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const int64_t* slots;
+  const int32_t* rows;                            /* [N], or null                 */
+  const float* k_descale_heads;                   /* e4m3: [Hkv], or null         */
+  const float* v_descale_heads;
+  float k_descale, v_descale;                     /* e4m3: times the above        */
+  int32_t* status;
+} AttnCacheAppend;
+ATTN_API int attn_cache_append(const AttnCacheAppend* desc, void* stream);
+
+/* Rotary positions with several axes (time, height, width; text has one).  Pair
+ * i of the first R values of a head turns by positions[axes[i]] * freqs[i]:
+ *   (x, y) -> (x cos - y sin, x sin + y cos),
+ * the pair being values (i, i + R/2), or (2i, 2i + 1) with `neighbours`; values
+ * R..D-1 are copied.  Angles are formed and reduced in 64 bits, so that far
+ * positions keep their phase.  `inverse` turns back, which is also the gradient.
+ * Q and K are [B, H, N, D] by strides (batch, head, token); either may be null.
+ * qo / ko may be q / k with the same strides. */
+typedef struct AttnRotary {
+  int32_t flags;
+  int32_t dtype;           /* ATTN_F32, ATTN_BF16 or ATTN_F16                     */
+  int32_t positions_64;    /* 0: positions are int32, 1: int64                    */
+  int32_t num_axes;
+  int32_t neighbours, inverse;
+  int64_t B, N, Hq, Hk, D, R;
+  int64_t q_stride[3], k_stride[3], qo_stride[3], ko_stride[3];
+  int64_t pos_stride[3];   /* axis, batch, token                                  */
+  const void* q;
+  const void* k;
+  void* qo;
+  void* ko;
+  const void* positions;   /* [num_axes, B, N]                                    */
+  const double* freqs;     /* [R/2] radians per position                          */
+  const int32_t* axes;     /* [R/2] axis of each pair, or null: all axis 0        */
+  int32_t* status;
+} AttnRotary;
+ATTN_API int attn_rotary(const AttnRotary* desc, void* stream);
+
+/* Attention of B requests' new tokens over the paged cache and over each other.
+ * The new tokens of request b are rows starts[b] .. starts[b+1]-1 of q, k_new
+ * and v_new (ragged, packed); it has lengths[b] cached tokens, all visible to
+ * them.  Among the new tokens of a request, token i sees token j unless
+ * mask[row of i][j] is non-zero; with no mask it sees j <= i (a chain: one
+ * token for decode, a chunk of a prompt).  With a mask, a drafted tree: mask
+ * out all but a node's ancestors and itself.
+ *   O = softmax(scale * q . k) . v over the visible keys,  LSE = ln of the sum
+ * A row that sees nothing gives O = 0 and LSE = -inf.  Rows of q past
+ * starts[B] are left as they were.  Keys and values of an e4m3 cache stand for
+ * themselves times the descales; k_new and v_new have q's type. */
+typedef struct AttnTree {
+  int32_t flags;
+  int32_t dtype;           /* q, k_new, v_new, o: ATTN_BF16 or ATTN_F16           */
+  int32_t cache_dtype;     /* the same, or ATTN_E4M3 (D = 128)                    */
+  int32_t page_size;
+  int64_t B, T, Hq, Hkv, D;
+  int64_t W, num_pages;    /* columns of block_table; pages of the cache          */
+  int64_t max_new;         /* no request has more new tokens than this            */
+  int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2];  /* token, head     */
+  int64_t k_cache_stride[3], v_cache_stride[3];                /* page, head, token */
+  int64_t table_stride;    /* elements between rows of block_table                */
+  int64_t mask_stride;     /* bytes between rows of mask (max_new columns)        */
+  const void* q;
+  const void* k_new;
+  const void* v_new;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  float* lse;              /* [T, Hq] fp32 contiguous, natural log, or null       */
+  const int32_t* block_table;  /* [B, W]                                          */
+  const int32_t* lengths;      /* [B]                                             */
+  const int32_t* starts;       /* [B + 1]                                         */
+  const uint8_t* mask;         /* [T, max_new], 1 = masked, or null               */
+  const float* k_descale_heads;  /* e4m3: [Hkv], or null                          */
+  const float* v_descale_heads;
+  float scale, k_descale, v_descale;
+  int32_t* status;
+} AttnTree;
+ATTN_API int attn_tree_fwd(const AttnTree* desc, void* stream);
 
 #ifdef __cplusplus
 }

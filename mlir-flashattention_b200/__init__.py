@@ -22,6 +22,7 @@ __all__ = [
     "AttentionError", "VerifyError", "fused", "classify_mask", "lib", "launch_count",
     "check_status", "AttnDesc", "AttnMemRef2D", "AttnMemRef4D", "memref", "shard_slices",
     "ATTN_F32", "ATTN_BF16", "ATTN_E4M3", "ATTN_F16", "MASK_NONE", "MASK_CAUSAL", "MASK_DENSE",
+    "cache_plan", "cache_append", "rotary_table", "rotary", "fused_tree", "CachePlan", "RotaryTable",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -34,6 +35,7 @@ STATUS = {
     0: "ok", -1: "invalid argument", -2: "shape mismatch", -3: "unsupported stride",
     -4: "unsupported dtype", -5: "misaligned pointer or stride", -6: "CUDA error",
     -7: "device wait timed out", -8: "unsupported variant", -9: "no sm_100 device",
+    -10: "capacity exceeded",
 }
 
 
@@ -78,6 +80,22 @@ class AttnMemRef4D(ctypes.Structure):
     _fields_ = [("allocated", ctypes.c_void_p), ("aligned", ctypes.c_void_p),
                 ("offset", ctypes.c_int64), ("sizes", ctypes.c_int64 * 4),
                 ("strides", ctypes.c_int64 * 4)]
+
+
+_SERVING = ("AttnCachePlan", "AttnCacheAppend", "AttnRotary", "AttnTree", "CachePlan", "RotaryTable",
+            "cache_plan", "cache_append", "rotary_table", "rotary", "fused_tree")
+
+
+def _serving():
+    from . import serving  # noqa: PLC0415  (needs torch, which this module only imports in calls)
+    return serving
+
+
+def __getattr__(name):
+    if name in _SERVING:
+        value = globals()[name] = getattr(_serving(), name)
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 _lib = None
@@ -203,7 +221,7 @@ def classify_mask(mask) -> int:
 
 def fused(Q, K, V, scale, mask=None, output=None, *, causal=False, lse=None,
           q_descale=1.0, k_descale=1.0, v_descale=1.0, stream=None, sync_check=False,
-          classify=True):
+          classify=True, rotary=None, positions=None):
     """Run ``attention.fused ins(Q, K, V) scale(scale) [mask(mask)] outs(output)``.
 
     Q: [Nq, D] or [B, Hq, Nq, D]; K, V: [Nk, D] or [B, Hkv, Nk, D] (Hq a
@@ -221,8 +239,14 @@ def fused(Q, K, V, scale, mask=None, output=None, *, causal=False, lse=None,
     block of Q), ``k_descale`` [B, Hkv, ceil(Nk/128)], ``v_descale`` [B, Hkv].
     ``classify=False`` runs a given mask on the dense-mask kernel as it is
     (no check for the causal or empty pattern).
+
+    ``rotary`` (a ``RotaryTable``) turns Q and K by ``positions`` (int32 or
+    int64 [axes, N] or [axes, B, N]) before they meet, on the same stream; Q
+    and K then have the same N and neither is e4m3.
     """
     import torch  # noqa: PLC0415
+    if rotary is not None or positions is not None:
+        Q, K = _turned(Q, K, rotary, positions, stream)
     q4 = _as4(Q, "Q", "seq_q", "head_dim")
     k4 = _as4(K, "K", "seq_k", "head_dim")
     v4 = _as4(V, "V", "seq_k", "head_dim")
@@ -306,6 +330,17 @@ def fused(Q, K, V, scale, mask=None, output=None, *, causal=False, lse=None,
         if sync_check:
             check_status(Q.device.index or 0, stream)
     return output
+
+
+def _turned(Q, K, table, positions, stream):
+    """Q and K of ``fused`` turned by their rotary positions."""
+    if table is None or positions is None:
+        raise VerifyError("rotary and positions go together")
+    q4, k4 = _as4(Q, "Q", "seq_q", "head_dim"), _as4(K, "K", "seq_k", "head_dim")
+    if q4.shape[2] != k4.shape[2]:
+        raise VerifyError("rotary positions need K seq_len equal to Q seq_len")
+    q, k = _serving().rotary(q4, k4, positions, table, stream=stream)
+    return q.reshape(Q.shape), k.reshape(K.shape)
 
 
 def memref(t, rank=None):

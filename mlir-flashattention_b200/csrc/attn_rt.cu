@@ -24,6 +24,7 @@
 #include "../../include/attn_rt.h"
 #include "attn_fwd_f32.cuh"
 #include "attn_fwd_sm100.cuh"
+#include "rt_host.h"
 
 namespace {
 
@@ -1181,7 +1182,7 @@ int run_views(int dtype, int out_dtype, int mask_kind, const View& Q, const View
 // =================================================================== C ABI
 extern "C" {
 
-int attn_rt_version(void) { return (1 << 16) | 1; }
+int attn_rt_version(void) { return (1 << 16) | 2; }
 
 int64_t attn_rt_launch_count(void) { return g_launches.load(); }
 
@@ -1226,6 +1227,7 @@ const char* attn_rt_status_string(int code) {
     case ATTN_ERR_TIMEOUT: return "device wait timed out";
     case ATTN_ERR_UNSUPPORTED: return "unsupported variant";
     case ATTN_ERR_NO_DEVICE: return "no sm_100 device";
+    case ATTN_ERR_CAPACITY: return "capacity exceeded";
     default: return "unknown status";
   }
 }
@@ -1593,3 +1595,28 @@ extern "C" int attn_fwd_host_noalloc(const AttnDesc* desc, void* stream_) {
   if (code != 0) return fail(code, "kernel reported %s", attn_rt_status_string(code));
   return ATTN_OK;
 }
+
+// ============================================== helpers of the serving calls
+namespace rt_host {
+
+int fail_with(int code, const char* message) { return fail(code, "%s", message); }
+
+int device_ready(Device* out) {
+  int dev = 0, rc;
+  if ((rc = current_device(&dev)) != ATTN_OK) return rc;
+  if ((rc = init_device(dev)) != ATTN_OK) return rc;
+  out->index = dev;
+  out->sms = g_dev[dev].sm_count;
+  out->status = g_dev[dev].status;
+  return ATTN_OK;
+}
+
+bool on_device(const void* p) { return is_device_ptr(p); }
+
+cudaError_t scratch(void** p, size_t bytes, cudaStream_t s) { return scratch_alloc(p, bytes, s); }
+
+void count_launches(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
+
+EncodeTiled tensor_map_encoder() { return encode_fn(); }
+
+}  // namespace rt_host

@@ -1,0 +1,425 @@
+// serve_rt.cu — host side of the serving calls in include/attn_rt.h: checks of
+// the descriptors, choice of kernel and launch.  No call waits for the device.
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+
+#include "attn_tree.cuh"
+#include "cache_append.cuh"
+#include "cache_plan.cuh"
+#include "rotary.cuh"
+#include "rt_host.h"
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return rt_host::fail_with(code, buf);
+}
+
+int cuda_fail(cudaError_t e, const char* what) {
+  return fail(ATTN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  rt_host::count_launches(1);
+  return ATTN_OK;
+}
+
+bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int page_shift(int page_size) {
+  for (int s = 4; s <= 10; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+
+int check_flags(int32_t flags) {
+  if (flags & ~ATTN_FLAG_DEVICE_POINTERS) return fail(ATTN_ERR_INVALID, "unknown flags 0x%x", flags);
+  return ATTN_OK;
+}
+
+// Kernels read these with TMA and plain loads: host memory would fault.
+template <size_t N>
+int check_pointers(int32_t flags, const void* const (&list)[N]) {
+  if (flags & ATTN_FLAG_DEVICE_POINTERS) return ATTN_OK;
+  for (const void* p : list)
+    if (p && !rt_host::on_device(p)) return fail(ATTN_ERR_INVALID, "serving calls take device pointers");
+  return ATTN_OK;
+}
+
+// A stride matters only along an extent of two or more.
+bool stride_ok(int64_t stride, int64_t extent, int64_t multiple) {
+  return extent <= 1 || stride % multiple == 0;
+}
+
+constexpr int64_t kInt32 = (int64_t{1} << 31) - 1;
+
+// ------------------------------------------------------------------- plan
+int check(const AttnCachePlan& d) {
+  int rc = check_flags(d.flags);
+  if (rc != ATTN_OK) return rc;
+  if (d.B < 0 || d.W < 0 || d.num_pages < 0 || d.tokens < 0)
+    return fail(ATTN_ERR_SHAPE, "extents must not be negative");
+  const int shift = page_shift(d.page_size);
+  if (shift < 0)
+    return fail(ATTN_ERR_UNSUPPORTED, "page_size must be a power of two from 16 to 1024 (got %d)",
+                d.page_size);
+  if (d.B > cache_plan::kMaxRequests)
+    return fail(ATTN_ERR_UNSUPPORTED, "at most %d requests a call (got %lld)",
+                cache_plan::kMaxRequests, (long long)d.B);
+  if (d.num_pages > kInt32 || d.tokens > kInt32 || d.W > kInt32 || (d.W << shift) > kInt32 ||
+      d.B * d.W > kInt32)
+    return fail(ATTN_ERR_SHAPE, "extent too large");
+  if (d.B > 1 && d.table_stride < d.W) return fail(ATTN_ERR_STRIDE, "block_table rows overlap");
+  if (!d.free_count || !d.free_count_out || !d.starts ||
+      (d.B > 0 && (!d.lengths || !d.targets || !d.lengths_out)) ||
+      (d.B > 0 && d.W > 0 && !d.block_table) || (d.num_pages > 0 && !d.free_pages) ||
+      (d.tokens > 0 && !d.slots))
+    return fail(ATTN_ERR_INVALID, "null pointer");
+  return ATTN_OK;
+}
+
+int run(const AttnCachePlan& d, cudaStream_t s) {
+  rt_host::Device dev;
+  int rc = rt_host::device_ready(&dev);
+  if (rc != ATTN_OK) return rc;
+  rc = check_pointers(d.flags, {d.lengths, d.targets, d.block_table, d.free_pages, d.free_count,
+                                d.lengths_out, d.free_count_out, d.starts, d.positions, d.slots,
+                                d.status});
+  if (rc != ATTN_OK) return rc;
+  cache_plan::Params p{};
+  p.B = static_cast<int>(d.B);
+  p.W = static_cast<int>(d.W);
+  p.page_shift = page_shift(d.page_size);
+  p.num_pages = static_cast<int>(d.num_pages);
+  p.tokens = static_cast<int>(d.tokens);
+  p.table_stride = d.table_stride;
+  p.lengths = d.lengths;
+  p.targets = d.targets;
+  p.table = d.block_table;
+  p.free_pages = d.free_pages;
+  p.free_count = d.free_count;
+  p.lengths_out = d.lengths_out;
+  p.free_count_out = d.free_count_out;
+  p.starts = d.starts;
+  p.positions = d.positions;
+  p.slots = d.slots;
+  p.status = d.status ? d.status : dev.status;
+  const size_t smem = (4 * static_cast<size_t>(d.B) + 3) * sizeof(int);
+  static std::once_flag once[64];
+  static cudaError_t attr[64];
+  std::call_once(once[dev.index], [&] {
+    attr[dev.index] = cudaFuncSetAttribute(cache_plan::plan_kernel,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (4 * cache_plan::kMaxRequests + 3) * int{sizeof(int)});
+  });
+  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "cudaFuncSetAttribute");
+  const int64_t work = std::max(d.B, d.tokens);
+  const int blocks = static_cast<int>(std::min<int64_t>(8, (work + 4095) / 4096));
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = static_cast<unsigned>(std::max(1, blocks));
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(at.val.clusterDim.x);
+  cfg.blockDim = dim3(work <= 256 ? 256 : 1024);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, cache_plan::plan_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "cache_plan launch");
+  rt_host::count_launches(1);
+  return ATTN_OK;
+}
+
+// ----------------------------------------------------------------- append
+int check(const AttnCacheAppend& d) {
+  int rc = check_flags(d.flags);
+  if (rc != ATTN_OK) return rc;
+  if (d.N < 0 || d.T < 0 || d.Hkv < 0 || d.D < 0 || d.num_pages < 0)
+    return fail(ATTN_ERR_SHAPE, "extents must not be negative");
+  if (d.dtype != ATTN_BF16 && d.dtype != ATTN_F16)
+    return fail(ATTN_ERR_DTYPE, "keys and values must be bf16 or f16");
+  if (d.cache_dtype != d.dtype && d.cache_dtype != ATTN_E4M3)
+    return fail(ATTN_ERR_DTYPE, "the cache must have the keys' type or e4m3");
+  if (page_shift(d.page_size) < 0)
+    return fail(ATTN_ERR_UNSUPPORTED, "page_size must be a power of two from 16 to 1024 (got %d)",
+                d.page_size);
+  if (d.D % 16 != 0)
+    return fail(ATTN_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 (got %lld)", (long long)d.D);
+  if (d.N > kInt32 || d.T > kInt32 || d.num_pages > kInt32 || d.Hkv * d.D > kInt32)
+    return fail(ATTN_ERR_SHAPE, "extent too large");
+  if (!d.rows && d.N > d.T)
+    return fail(ATTN_ERR_SHAPE, "more slots (%lld) than rows (%lld)", (long long)d.N, (long long)d.T);
+  if (d.N == 0 || d.Hkv == 0 || d.D == 0) return ATTN_OK;
+  if (!d.slots || (d.T > 0 && (!d.k || !d.v)) || (d.num_pages > 0 && (!d.k_cache || !d.v_cache)))
+    return fail(ATTN_ERR_INVALID, "null pointer");
+  const bool fp8 = d.cache_dtype == ATTN_E4M3;
+  if (fp8 && !(d.k_descale > 0.f && d.v_descale > 0.f && std::isfinite(d.k_descale) &&
+               std::isfinite(d.v_descale)))
+    return fail(ATTN_ERR_INVALID, "e4m3 descales must be positive and finite");
+  if (!fp8 && (d.k_descale_heads || d.v_descale_heads || d.k_descale != 1.f || d.v_descale != 1.f))
+    return fail(ATTN_ERR_DTYPE, "descales apply to e4m3 caches only");
+  const int64_t ca = fp8 ? 16 : 8;
+  for (const void* ptr : {d.k, d.v, static_cast<const void*>(d.k_cache), static_cast<const void*>(d.v_cache)})
+    if (!aligned(ptr, 16)) return fail(ATTN_ERR_ALIGN, "keys, values and caches must be 16-byte aligned");
+  for (const int64_t* st : {d.k_stride, d.v_stride})
+    if (!stride_ok(st[0], d.T, 8) || !stride_ok(st[1], d.Hkv, 8))
+      return fail(ATTN_ERR_ALIGN, "strides of keys and values must be multiples of 16 bytes");
+  for (const int64_t* st : {d.k_cache_stride, d.v_cache_stride})
+    if (!stride_ok(st[0], d.num_pages, ca) || !stride_ok(st[1], d.Hkv, ca) || st[2] % ca != 0)
+      return fail(ATTN_ERR_ALIGN, "cache strides must be multiples of 16 bytes");
+  return ATTN_OK;
+}
+
+int run(const AttnCacheAppend& d, cudaStream_t s) {
+  if (d.N == 0 || d.Hkv == 0 || d.D == 0) return ATTN_OK;
+  rt_host::Device dev;
+  int rc = rt_host::device_ready(&dev);
+  if (rc != ATTN_OK) return rc;
+  rc = check_pointers(d.flags, {d.k, d.v, d.k_cache, d.v_cache, d.slots, d.rows, d.k_descale_heads,
+                                d.v_descale_heads, d.status});
+  if (rc != ATTN_OK) return rc;
+  cache_append::Params p{};
+  p.N = d.N;
+  p.T = d.T;
+  p.page_shift = page_shift(d.page_size);
+  p.slots_in_cache = d.num_pages << p.page_shift;
+  p.Hkv = static_cast<int>(d.Hkv);
+  p.chunks = static_cast<int>(d.D / 16);
+  p.k_st = d.k_stride[0], p.k_sh = d.k_stride[1];
+  p.v_st = d.v_stride[0], p.v_sh = d.v_stride[1];
+  p.kc_sp = d.k_cache_stride[0], p.kc_sh = d.k_cache_stride[1], p.kc_st = d.k_cache_stride[2];
+  p.vc_sp = d.v_cache_stride[0], p.vc_sh = d.v_cache_stride[1], p.vc_st = d.v_cache_stride[2];
+  p.k = d.k, p.v = d.v, p.kc = d.k_cache, p.vc = d.v_cache;
+  p.slots = d.slots;
+  p.rows = d.rows;
+  p.k_descale_heads = d.k_descale_heads, p.v_descale_heads = d.v_descale_heads;
+  p.k_descale = d.k_descale, p.v_descale = d.v_descale;
+  p.status = d.status ? d.status : dev.status;
+  const int64_t units = d.N * p.Hkv * p.chunks * 2;
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, dev.sms * 64));
+  const bool fp8 = d.cache_dtype == ATTN_E4M3;
+  auto kern = d.dtype == ATTN_F16
+                  ? (fp8 ? cache_append::append_kernel<true, true> : cache_append::append_kernel<true, false>)
+                  : (fp8 ? cache_append::append_kernel<false, true>
+                         : cache_append::append_kernel<false, false>);
+  kern<<<blocks, 256, 0, s>>>(p);
+  return launched("cache_append launch");
+}
+
+// ----------------------------------------------------------------- rotary
+int check(const AttnRotary& d) {
+  int rc = check_flags(d.flags);
+  if (rc != ATTN_OK) return rc;
+  if (d.B < 0 || d.N < 0 || d.Hq < 0 || d.Hk < 0 || d.D < 0 || d.R < 0)
+    return fail(ATTN_ERR_SHAPE, "extents must not be negative");
+  if (d.dtype != ATTN_F32 && d.dtype != ATTN_BF16 && d.dtype != ATTN_F16)
+    return fail(ATTN_ERR_DTYPE, "rotary takes f32, bf16 or f16");
+  if (d.R % 2 != 0 || d.R > d.D)
+    return fail(ATTN_ERR_SHAPE, "the turned values must be an even number up to head_dim (%lld of %lld)",
+                (long long)d.R, (long long)d.D);
+  if (d.D > 1024) return fail(ATTN_ERR_UNSUPPORTED, "rotary supports head_dim <= 1024");
+  if (d.num_axes < 1) return fail(ATTN_ERR_SHAPE, "positions need an axis");
+  if (d.N > kInt32 || d.B > kInt32 || d.B * d.N > kInt32 || (d.Hq + d.Hk) * d.D > kInt32)
+    return fail(ATTN_ERR_SHAPE, "extent too large");
+  if (d.B * d.N == 0 || (d.Hq + d.Hk) * d.D == 0) return ATTN_OK;
+  if ((d.Hq > 0 && (!d.q || !d.qo)) || (d.Hk > 0 && (!d.k || !d.ko)) ||
+      (d.R > 0 && (!d.positions || !d.freqs)))
+    return fail(ATTN_ERR_INVALID, "null pointer");
+  const unsigned eb = d.dtype == ATTN_F32 ? 4 : 2;
+  for (const void* ptr : {d.q, d.k, static_cast<const void*>(d.qo), static_cast<const void*>(d.ko)})
+    if (!aligned(ptr, eb)) return fail(ATTN_ERR_ALIGN, "Q and K must be aligned to their elements");
+  return ATTN_OK;
+}
+
+template <typename T, int V>
+int launch_rotary(const AttnRotary& d, const rotary::Params& p, cudaStream_t s) {
+  const unsigned blocks = static_cast<unsigned>((p.tokens + p.tile - 1) / p.tile);
+  const size_t smem = sizeof(float2) * p.tile * p.half;
+  if (d.neighbours)
+    rotary::rotary_kernel<T, V, true><<<blocks, rotary::kThreads, smem, s>>>(p);
+  else
+    rotary::rotary_kernel<T, V, false><<<blocks, rotary::kThreads, smem, s>>>(p);
+  return launched("rotary launch");
+}
+
+int run(const AttnRotary& d, cudaStream_t s) {
+  if (d.B * d.N == 0 || (d.Hq + d.Hk) * d.D == 0) return ATTN_OK;
+  rt_host::Device dev;
+  int rc = rt_host::device_ready(&dev);
+  if (rc != ATTN_OK) return rc;
+  rc = check_pointers(d.flags, {d.Hq ? d.q : nullptr, d.Hk ? d.k : nullptr, d.Hq ? d.qo : nullptr,
+                                d.Hk ? d.ko : nullptr, d.positions, d.freqs, d.axes, d.status});
+  if (rc != ATTN_OK) return rc;
+  rotary::Params p{};
+  p.tokens = d.B * d.N;
+  p.N = d.N;
+  p.Hq = static_cast<int>(d.Hq);
+  p.H = static_cast<int>(d.Hq + d.Hk);
+  p.D = static_cast<int>(d.D);
+  p.half = static_cast<int>(d.R / 2);
+  p.q_sb = d.q_stride[0], p.q_sh = d.q_stride[1], p.q_sn = d.q_stride[2];
+  p.k_sb = d.k_stride[0], p.k_sh = d.k_stride[1], p.k_sn = d.k_stride[2];
+  p.qo_sb = d.qo_stride[0], p.qo_sh = d.qo_stride[1], p.qo_sn = d.qo_stride[2];
+  p.ko_sb = d.ko_stride[0], p.ko_sh = d.ko_stride[1], p.ko_sn = d.ko_stride[2];
+  p.p_sa = d.pos_stride[0], p.p_sb = d.pos_stride[1], p.p_sn = d.pos_stride[2];
+  p.q = d.q, p.k = d.k, p.qo = d.qo, p.ko = d.ko;
+  p.positions = d.positions;
+  p.freqs = d.freqs;
+  p.axes = d.axes;
+  p.status = d.status ? d.status : dev.status;
+  p.num_axes = d.num_axes;
+  p.positions_64 = d.positions_64;
+  p.sign = d.inverse ? -1.f : 1.f;
+  // 16-byte packs where every row, its second half and its tail allow them.
+  const int eb = d.dtype == ATTN_F32 ? 4 : 2, vec = 16 / eb;
+  bool wide = p.D % vec == 0 && p.half % vec == 0;
+  struct { const void* ptr; const int64_t* st; int64_t heads; } ops[] = {
+      {d.q, d.q_stride, d.Hq}, {d.qo, d.qo_stride, d.Hq}, {d.k, d.k_stride, d.Hk}, {d.ko, d.ko_stride, d.Hk}};
+  for (const auto& o : ops)
+    if (o.heads > 0)
+      wide = wide && aligned(o.ptr, 16) && stride_ok(o.st[0], d.B, vec) && stride_ok(o.st[1], o.heads, vec) &&
+             stride_ok(o.st[2], d.N, vec);
+  // Tokens per block: about two packs a thread, and angles within 32 KB.
+  const int per_token = p.H * (p.D - p.half) / (wide ? vec : 1);
+  p.tile = std::max(1, 2 * rotary::kThreads / std::max(1, per_token));
+  if (p.half > 0) p.tile = std::max(1, std::min(p.tile, 4096 / p.half));
+  switch (d.dtype) {
+    case ATTN_F32: return wide ? launch_rotary<float, 4>(d, p, s) : launch_rotary<float, 1>(d, p, s);
+    case ATTN_F16: return wide ? launch_rotary<__half, 8>(d, p, s) : launch_rotary<__half, 1>(d, p, s);
+    default:
+      return wide ? launch_rotary<__nv_bfloat16, 8>(d, p, s) : launch_rotary<__nv_bfloat16, 1>(d, p, s);
+  }
+}
+
+// ------------------------------------------------------------------- tree
+int check(const AttnTree& d) {
+  int rc = check_flags(d.flags);
+  if (rc != ATTN_OK) return rc;
+  if (d.B < 0 || d.T < 0 || d.Hq < 0 || d.Hkv < 0 || d.W < 0 || d.num_pages < 0 || d.max_new < 0)
+    return fail(ATTN_ERR_SHAPE, "extents must not be negative");
+  if (d.dtype != ATTN_BF16 && d.dtype != ATTN_F16)
+    return fail(ATTN_ERR_DTYPE, "queries must be bf16 or f16");
+  if (d.cache_dtype != d.dtype && d.cache_dtype != ATTN_E4M3)
+    return fail(ATTN_ERR_DTYPE, "the cache must have the queries' type or e4m3");
+  const int shift = page_shift(d.page_size);
+  if (shift < 0)
+    return fail(ATTN_ERR_UNSUPPORTED, "page_size must be a power of two from 16 to 1024 (got %d)",
+                d.page_size);
+  if (d.cache_dtype == ATTN_E4M3 ? d.D != 128 : (d.D != 64 && d.D != 128))
+    return fail(ATTN_ERR_UNSUPPORTED, "head_dim must be 64 or 128, with an e4m3 cache 128 (got %lld)",
+                (long long)d.D);
+  if (d.Hq > 0 && (d.Hkv <= 0 || d.Hq % d.Hkv != 0))
+    return fail(ATTN_ERR_SHAPE, "query heads (%lld) must be a multiple of key/value heads (%lld)",
+                (long long)d.Hq, (long long)d.Hkv);
+  if (d.Hq > 0 && d.Hq / d.Hkv > 64)
+    return fail(ATTN_ERR_UNSUPPORTED, "at most 64 query heads share a key head (got %lld)",
+                (long long)(d.Hq / d.Hkv));
+  if (d.B > 65535 || d.T > kInt32 || d.Hq > 65535 || d.max_new > kInt32 || d.num_pages > kInt32 ||
+      d.W > kInt32 || (d.W << shift) > kInt32 || d.T * d.Hq > kInt32)
+    return fail(ATTN_ERR_SHAPE, "extent too large");
+  if (d.B == 0 || d.T == 0 || d.Hq == 0 || d.max_new == 0) return ATTN_OK;
+  if (!d.q || !d.k_new || !d.v_new || !d.o || !d.lengths || !d.starts ||
+      (d.W > 0 && !d.block_table) || (d.num_pages > 0 && (!d.k_cache || !d.v_cache)))
+    return fail(ATTN_ERR_INVALID, "null pointer");
+  if (d.B > 1 && d.table_stride < d.W) return fail(ATTN_ERR_STRIDE, "block_table rows overlap");
+  if (d.mask && d.T > 1 && d.mask_stride < d.max_new)
+    return fail(ATTN_ERR_STRIDE, "mask rows must hold max_new columns");
+  if (!std::isfinite(d.scale)) return fail(ATTN_ERR_INVALID, "scale must be finite");
+  const bool fp8 = d.cache_dtype == ATTN_E4M3;
+  if (fp8 && !(d.k_descale > 0.f && d.v_descale > 0.f && std::isfinite(d.k_descale) &&
+               std::isfinite(d.v_descale)))
+    return fail(ATTN_ERR_INVALID, "e4m3 descales must be positive and finite");
+  if (!fp8 && (d.k_descale_heads || d.v_descale_heads || d.k_descale != 1.f || d.v_descale != 1.f))
+    return fail(ATTN_ERR_DTYPE, "descales apply to e4m3 caches only");
+  for (const void* ptr : {d.q, d.k_new, d.v_new, d.k_cache, d.v_cache, static_cast<const void*>(d.o)})
+    if (!aligned(ptr, 16)) return fail(ATTN_ERR_ALIGN, "queries, keys, values and output must be 16-byte aligned");
+  struct { const int64_t* st; int64_t heads; } rows[] = {
+      {d.q_stride, d.Hq}, {d.k_stride, d.Hkv}, {d.v_stride, d.Hkv}, {d.o_stride, d.Hq}};
+  for (const auto& r : rows)
+    if (!stride_ok(r.st[0], d.T, 8) || !stride_ok(r.st[1], r.heads, 8))
+      return fail(ATTN_ERR_ALIGN, "strides must be multiples of 16 bytes");
+  const int64_t ca = fp8 ? 16 : 8;
+  for (const int64_t* st : {d.k_cache_stride, d.v_cache_stride})
+    if (!stride_ok(st[0], d.num_pages, ca) || !stride_ok(st[1], d.Hkv, ca) || st[2] % ca != 0)
+      return fail(ATTN_ERR_ALIGN, "cache strides must be multiples of 16 bytes");
+  return ATTN_OK;
+}
+
+template <typename T, typename TC, int D>
+int launch_tree(const attn_tree::Params& p, cudaStream_t s) {
+  attn_tree::tree_kernel<T, TC, D><<<dim3(p.T, p.Hq), 128, 0, s>>>(p);
+  return launched("attn_tree launch");
+}
+
+int run(const AttnTree& d, cudaStream_t s) {
+  if (d.B == 0 || d.T == 0 || d.Hq == 0 || d.max_new == 0) return ATTN_OK;
+  rt_host::Device dev;
+  int rc = rt_host::device_ready(&dev);
+  if (rc != ATTN_OK) return rc;
+  rc = check_pointers(d.flags, {d.q, d.k_new, d.v_new, d.k_cache, d.v_cache, d.o, d.lse, d.block_table,
+                                d.lengths, d.starts, d.mask, d.k_descale_heads, d.v_descale_heads,
+                                d.status});
+  if (rc != ATTN_OK) return rc;
+  attn_tree::Params p{};
+  p.B = static_cast<int>(d.B);
+  p.T = static_cast<int>(d.T);
+  p.Hq = static_cast<int>(d.Hq);
+  p.Hkv = static_cast<int>(d.Hkv);
+  p.group = static_cast<int>(d.Hq / d.Hkv);
+  p.W = static_cast<int>(d.W);
+  p.num_pages = static_cast<int>(d.num_pages);
+  p.page_shift = page_shift(d.page_size);
+  p.max_new = static_cast<int>(std::min(d.max_new, d.T));
+  p.q_st = d.q_stride[0], p.q_sh = d.q_stride[1];
+  p.k_st = d.k_stride[0], p.k_sh = d.k_stride[1];
+  p.v_st = d.v_stride[0], p.v_sh = d.v_stride[1];
+  p.o_st = d.o_stride[0], p.o_sh = d.o_stride[1];
+  p.kc_sp = d.k_cache_stride[0], p.kc_sh = d.k_cache_stride[1], p.kc_st = d.k_cache_stride[2];
+  p.vc_sp = d.v_cache_stride[0], p.vc_sh = d.v_cache_stride[1], p.vc_st = d.v_cache_stride[2];
+  p.table_stride = d.table_stride;
+  p.mask_stride = d.mask_stride;
+  p.q = d.q, p.k_new = d.k_new, p.v_new = d.v_new;
+  p.k_cache = d.k_cache, p.v_cache = d.v_cache;
+  p.o = d.o, p.lse = d.lse;
+  p.table = d.block_table, p.lengths = d.lengths, p.starts = d.starts, p.mask = d.mask;
+  p.k_descale_heads = d.k_descale_heads, p.v_descale_heads = d.v_descale_heads;
+  p.scale = d.scale, p.k_descale = d.k_descale, p.v_descale = d.v_descale;
+  p.status = d.status ? d.status : dev.status;
+  using H = __half;
+  using N = __nv_bfloat16;
+  using E = __nv_fp8_e4m3;
+  const bool fp8 = d.cache_dtype == ATTN_E4M3;
+  if (d.dtype == ATTN_F16)
+    return fp8 ? launch_tree<H, E, 128>(p, s) : d.D == 64 ? launch_tree<H, H, 64>(p, s) : launch_tree<H, H, 128>(p, s);
+  return fp8 ? launch_tree<N, E, 128>(p, s) : d.D == 64 ? launch_tree<N, N, 64>(p, s) : launch_tree<N, N, 128>(p, s);
+}
+
+template <typename Desc>
+int call(const Desc* desc, void* stream) {
+  if (!desc) return fail(ATTN_ERR_INVALID, "null descriptor");
+  const int rc = check(*desc);
+  return rc != ATTN_OK ? rc : run(*desc, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+int attn_cache_plan(const AttnCachePlan* desc, void* stream) { return call(desc, stream); }
+int attn_cache_append(const AttnCacheAppend* desc, void* stream) { return call(desc, stream); }
+int attn_rotary(const AttnRotary* desc, void* stream) { return call(desc, stream); }
+int attn_tree_fwd(const AttnTree* desc, void* stream) { return call(desc, stream); }
+
+}  // extern "C"
