@@ -5,6 +5,10 @@
 // over the cached keys j < lengths[b] and the request's new keys that the mask
 // leaves visible, by the online recurrence with a running maximum m, sum l and
 // accumulator in 32 bits.
+//
+// This header: what the kernels share - operands, the requests as the device
+// arrays give them, and the split of the work.  attn_tree_mma.cuh holds the
+// kernel for few query rows and the join of split items.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -19,6 +23,7 @@ namespace attn_tree {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
+constexpr uint64_t kWaitLimitNs = 1000000000ull;  // 1 s per wait
 
 struct Params {
   int B, T, Hq, Hkv, group;
@@ -64,96 +69,186 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   return r;
 }
 
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f(__nv_fp8_e4m3 x) { return static_cast<float>(x); }
+// ----------------------------------------------------------------- the work
+// An item is one tile of query rows of one request and kv-head: row r of the
+// request is its token r / group with the kv-head's q-head r % group, so that
+// the heads that share keys share the tile.  Its units are tiles of keys: the
+// cached ones in order, then the new ones it can see.  The units of all items,
+// one after another, are cut into one equal share per block whatever the
+// requests' lengths; a share may begin and end inside an item.  A block meets
+// its share as pieces; one that is not a whole item goes to scratch, and the
+// join (a second kernel) adds up the pieces of each cut item in order.
+struct Split {
+  int rows;        // query rows of a tile
+  int keys_shift;  // cached keys of a tile, log2
+  int new_shift;   // new keys of a tile, log2
+};
+
+struct Piece {
+  int b, h, rt;       // request, kv-head, row tile
+  int k0, k1, tiles;  // units [k0, k1) of the item's `tiles`
+  int cached;         // how many of the item's tiles are cached keys
+  Request r;
+};
+
+// The new-key tiles that row tile rt of a request sees.
+__device__ __forceinline__ int new_tiles(const Params& p, const Split& s, const Request& r, int rt) {
+  int keys = r.count;
+  if (p.mask == nullptr) keys = min(keys, (rt * s.rows + s.rows - 1) / p.group + 1);
+  return (keys + (1 << s.new_shift) - 1) >> s.new_shift;
+}
+
+__device__ __forceinline__ int cached_tiles(const Split& s, const Request& r) {
+  return (r.held + (1 << s.keys_shift) - 1) >> s.keys_shift;
+}
+
+__device__ __forceinline__ int row_tiles(const Params& p, const Split& s, const Request& r) {
+  return static_cast<int>((static_cast<int64_t>(r.count) * p.group + s.rows - 1) / s.rows);
+}
+
+// Units of one kv-head of a request.
+__device__ __forceinline__ int64_t head_units(const Params& p, const Split& s, const Request& r) {
+  const int rts = row_tiles(p, s, r);
+  if (rts == 0) return 0;
+  int64_t u = static_cast<int64_t>(rts) * cached_tiles(s, r);
+  if (p.mask || rts == 1) return u + static_cast<int64_t>(rts) * new_tiles(p, s, r, rts - 1);
+  for (int rt = 0; rt < rts; ++rt) u += new_tiles(p, s, r, rt);
+  return u;
+}
+
+// Where a block's share begins, found by the whole block (blockDim.x threads,
+// a multiple of 32, at most 1024).
+struct Share {
+  int64_t lo, hi;  // units of this block
+  int64_t base;    // units before request b
+  int b;           // request that holds unit lo
+};
+
+__device__ __forceinline__ Share find_share(const Params& p, const Split& s, int min_units) {
+  __shared__ int64_t warp_sum[32];
+  __shared__ int64_t found_base;
+  __shared__ int found_b;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  auto units = [&](int b) -> int64_t {
+    return b < p.B ? head_units(p, s, request(p, b)) * p.Hkv : 0;
+  };
+  auto scan = [&](int64_t v) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t t = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += t;
+    }
+    return v;
+  };
+  const int chunks = (p.B + blockDim.x - 1) / blockDim.x;
+  int64_t mine = 0, inc = 0;
+  for (int c = 0; c < chunks; ++c) {
+    const int64_t u = units(c * blockDim.x + tid);
+    if (chunks == 1) inc = scan(u);
+    mine += u;
+  }
+  const int64_t sum = chunks == 1 ? inc : scan(mine);
+  if (lane == 31) warp_sum[warp] = sum;
+  __syncthreads();
+  int64_t total = 0, before = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  Share r;
+  const int64_t blocks = min(static_cast<int64_t>(gridDim.x), (total + min_units - 1) / min_units);
+  const int64_t c = blockIdx.x;
+  if (c >= blocks) {
+    r.lo = r.hi = r.base = 0;
+    r.b = 0;
+    return r;
+  }
+  r.lo = total * c / blocks;
+  r.hi = total * (c + 1) / blocks;
+  if (chunks == 1) {
+    const int64_t end = before + inc, start = end - mine;
+    if (start <= r.lo && r.lo < end) {
+      found_base = start;
+      found_b = tid;
+    }
+  } else {
+    int64_t run = 0;
+    for (int ch = 0; ch < chunks; ++ch) {
+      const int b = ch * blockDim.x + tid;
+      const int64_t u = units(b), in = scan(u);
+      __syncthreads();
+      if (lane == 31) warp_sum[warp] = in;
+      __syncthreads();
+      int64_t pre = run;
+      for (int w = 0; w < warps; ++w) {
+        if (w < warp) pre += warp_sum[w];
+        run += warp_sum[w];
+      }
+      const int64_t end = pre + in, start = end - u;
+      if (start <= r.lo && r.lo < end) {
+        found_base = start;
+        found_b = b;
+      }
+    }
+  }
+  __syncthreads();
+  r.base = found_base;
+  r.b = found_b;
+  return r;
+}
+
+// The next piece of a share; moves lo past it.  False at its end.
+__device__ __forceinline__ bool next_piece(const Params& p, const Split& s, Share& sh, Piece& out) {
+  if (sh.lo >= sh.hi) return false;
+  Request r;
+  int64_t uh;
+  while (true) {
+    if (sh.b >= p.B) return false;  // lengths changed under the call
+    r = request(p, sh.b);
+    uh = head_units(p, s, r);
+    if (sh.lo - sh.base < uh * p.Hkv) break;
+    sh.base += uh * p.Hkv;
+    ++sh.b;
+  }
+  int64_t off = sh.lo - sh.base;
+  out.b = sh.b;
+  out.r = r;
+  out.h = static_cast<int>(off / uh);
+  off -= out.h * uh;
+  out.cached = cached_tiles(s, r);
+  if (p.mask || row_tiles(p, s, r) == 1) {
+    out.tiles = out.cached + new_tiles(p, s, r, row_tiles(p, s, r) - 1);
+    out.rt = static_cast<int>(off / out.tiles);
+    off -= static_cast<int64_t>(out.rt) * out.tiles;
+  } else {
+    for (out.rt = 0;; ++out.rt) {
+      out.tiles = out.cached + new_tiles(p, s, r, out.rt);
+      if (off < out.tiles) break;
+      off -= out.tiles;
+    }
+  }
+  out.k0 = static_cast<int>(off);
+  out.k1 = static_cast<int>(min(static_cast<int64_t>(out.tiles), off + (sh.hi - sh.lo)));
+  sh.lo += out.k1 - out.k0;
+  return true;
+}
+
+// Scratch of the pieces that are not whole items: block c's first piece goes
+// to slot 2 c, its last to 2 c + 1.
+struct Record {
+  int b, h, rt;  // b = -1: nothing in this slot
+  int ends;      // bit 0: the item's first piece, bit 1: its last
+};
+
+struct Scratch {
+  Record* record;  // [2 blocks]
+  float* m;        // [2 blocks][rows] running maximum, log2 units
+  float* l;        // [2 blocks][rows]
+  float* o;        // [2 blocks][rows][D], relative to m, not divided by l
+};
+
 template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
-
-// One block per (row of q, q-head): 4 warps take keys in turn, a key at a time
-// per warp, and are joined at the end.
-template <typename T, typename TC, int D>
-__global__ void __launch_bounds__(128) tree_kernel(const Params p) {
-  constexpr int E = D / 32;
-  __shared__ float sh_m[4], sh_l[4], sh_o[4][D];
-  const int t = blockIdx.x, h = blockIdx.y, hk = h / p.group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int b = -1;
-  Request r{};
-  for (int i = 0; i < p.B; ++i) {
-    r = request(p, i);
-    if (t >= r.first && t < r.first + r.count) {
-      b = i;
-      break;
-    }
-  }
-  if (b < 0) return;
-  const int i = t - r.first;
-  float q[E], o[E] = {};
-  for (int e = 0; e < E; ++e)
-    q[e] = to_f(static_cast<const T*>(p.q)[t * p.q_st + h * p.q_sh + lane + 32 * e]);
-  const float kd = p.k_descale * (p.k_descale_heads ? p.k_descale_heads[hk] : 1.f);
-  const float vd = p.v_descale * (p.v_descale_heads ? p.v_descale_heads[hk] : 1.f);
-  float m = -INFINITY, l = 0.f;
-  auto step = [&](const float (&k)[E], const float (&v)[E]) {
-    float s = 0.f;
-    for (int e = 0; e < E; ++e) s += q[e] * k[e];
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= p.scale * kLog2e;
-    const float top = fmaxf(m, s);
-    if (top == -INFINITY) return;
-    const float a = exp2f(m - top), w = exp2f(s - top);
-    l = l * a + w;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * v[e];
-    m = top;
-  };
-  float k[E], v[E];
-  for (int j = warp; j < r.held; j += 4) {
-    const int page = p.table[b * p.table_stride + (j >> p.page_shift)];
-    const int at = j & ((1 << p.page_shift) - 1);
-    if (page < 0 || page >= p.num_pages) {
-      atomicCAS(p.status, 0, ATTN_ERR_INVALID);
-      continue;
-    }
-    const TC* kp = static_cast<const TC*>(p.k_cache) + page * p.kc_sp + hk * p.kc_sh + at * p.kc_st;
-    const TC* vp = static_cast<const TC*>(p.v_cache) + page * p.vc_sp + hk * p.vc_sh + at * p.vc_st;
-    for (int e = 0; e < E; ++e) {
-      k[e] = to_f(kp[lane + 32 * e]) * kd;
-      v[e] = to_f(vp[lane + 32 * e]) * vd;
-    }
-    step(k, v);
-  }
-  for (int j = warp; j < r.count; j += 4) {
-    if (p.mask ? p.mask[t * p.mask_stride + j] != 0 : j > i) continue;
-    const T* kp = static_cast<const T*>(p.k_new) + (r.first + j) * p.k_st + hk * p.k_sh;
-    const T* vp = static_cast<const T*>(p.v_new) + (r.first + j) * p.v_st + hk * p.v_sh;
-    for (int e = 0; e < E; ++e) {
-      k[e] = to_f(kp[lane + 32 * e]);
-      v[e] = to_f(vp[lane + 32 * e]);
-    }
-    step(k, v);
-  }
-  if (lane == 0) {
-    sh_m[warp] = m;
-    sh_l[warp] = l;
-  }
-  for (int e = 0; e < E; ++e) sh_o[warp][lane + 32 * e] = o[e];
-  __syncthreads();
-  const float top = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
-  float a[4], sum = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    a[w] = top == -INFINITY ? 0.f : exp2f(sh_m[w] - top);
-    sum += a[w] * sh_l[w];
-  }
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float x = 0.f;
-    for (int w = 0; w < 4; ++w) x += a[w] * sh_o[w][d];
-    static_cast<T*>(p.o)[t * p.o_st + h * p.o_sh + d] = from_f<T>(sum > 0.f ? x / sum : 0.f);
-  }
-  if (p.lse && threadIdx.x == 0)
-    p.lse[static_cast<int64_t>(t) * p.Hq + h] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
-}
 
 }  // namespace attn_tree

@@ -6,7 +6,7 @@
 #include <cstdio>
 #include <mutex>
 
-#include "attn_tree.cuh"
+#include "attn_tree_mma.cuh"
 #include "cache_append.cuh"
 #include "cache_plan.cuh"
 #include "rotary.cuh"
@@ -357,10 +357,119 @@ int check(const AttnTree& d) {
   return ATTN_OK;
 }
 
+// 5-D tensor map of an operand seen as [pages][heads][halves][tokens][128 bytes]
+// (new tokens: one page), with a box of `box_rows` tokens of one head.
+int make_map(CUtensorMap* map, const void* base, int type_bytes, CUtensorMapDataType type, int64_t D,
+             int64_t tokens, int64_t heads, int64_t pages, int64_t s_token, int64_t s_head, int64_t s_page,
+             int box_rows) {
+  const rt_host::EncodeTiled encode = rt_host::tensor_map_encoder();
+  if (!encode) return fail(ATTN_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  // Strides along an extent of one are never stepped along.
+  if (tokens == 1) s_token = D;
+  if (heads == 1) s_head = s_token * tokens;
+  if (pages == 1) s_page = s_head * heads;
+  const cuuint64_t halves = static_cast<cuuint64_t>(D * type_bytes / 128);
+  const cuuint64_t inner = 128 / type_bytes;
+  const cuuint64_t dims[5] = {inner, static_cast<cuuint64_t>(tokens), halves, static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(pages)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(s_token * type_bytes), 128,
+                                 static_cast<cuuint64_t>(s_head * type_bytes),
+                                 static_cast<cuuint64_t>(s_page * type_bytes)};
+  for (cuuint64_t s : strides)
+    if (s % 16 != 0 || s >= (1ull << 40)) return fail(ATTN_ERR_STRIDE, "a stride is negative or past 2^40 bytes");
+  const cuuint32_t box[5] = {static_cast<cuuint32_t>(inner), static_cast<cuuint32_t>(box_rows),
+                             static_cast<cuuint32_t>(halves), 1, 1};
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(map, type, 5, const_cast<void*>(base), dims, strides, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ATTN_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return ATTN_OK;
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Scratch for the cut items of a launch of `blocks` blocks.
+int tree_scratch(attn_tree::Scratch* out, void** base, int blocks, int rows, int D, cudaStream_t s) {
+  const size_t slots = 2 * static_cast<size_t>(blocks);
+  const size_t rec = round256(slots * sizeof(attn_tree::Record)), ml = round256(slots * rows * sizeof(float));
+  const cudaError_t e = rt_host::scratch(base, rec + 2 * ml + slots * rows * D * sizeof(float), s);
+  if (e != cudaSuccess) return cuda_fail(e, "stream-ordered scratch (cut items)");
+  char* at = static_cast<char*>(*base);
+  out->record = reinterpret_cast<attn_tree::Record*>(at);
+  out->m = reinterpret_cast<float*>(at + rec);
+  out->l = reinterpret_cast<float*>(at + rec + ml);
+  out->o = reinterpret_cast<float*>(at + rec + 2 * ml);
+  return ATTN_OK;
+}
+
+// The join, launched so that it is set up while the first kernel still runs.
+template <typename T, int D, int ROWS>
+cudaError_t launch_join(const attn_tree::Params& p, const attn_tree::Scratch& sc, float shift, int blocks,
+                        cudaStream_t s) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(attn_tree::kJoinThreads);
+  cfg.dynamicSmemBytes = sizeof(float) * blocks * ROWS;
+  cfg.stream = s;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_tree::tree_join_kernel<T, D, ROWS>, p, sc, shift);
+}
+
+int pow2_shift(int64_t n, int lo, int hi) {
+  int s = lo;
+  while (s < hi && (int64_t{1} << s) < n) ++s;
+  return s;
+}
+
 template <typename T, typename TC, int D>
-int launch_tree(const attn_tree::Params& p, cudaStream_t s) {
-  attn_tree::tree_kernel<T, TC, D><<<dim3(p.T, p.Hq), 128, 0, s>>>(p);
-  return launched("attn_tree launch");
+int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, int sms, int device, cudaStream_t s) {
+  using C = attn_tree::MmaCfg<T, TC, D>;
+  constexpr int kRows = attn_tree::kMmaRows;
+  auto kern = attn_tree::tree_mma_kernel<T, TC, D>;
+  static std::once_flag once[64];
+  static cudaError_t attr[64];
+  std::call_once(once[device], [&] {
+    attr[device] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
+  });
+  if (attr[device] != cudaSuccess) return cuda_fail(attr[device], "cudaFuncSetAttribute");
+  const CUtensorMapDataType t16 = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapDataType tc = C::FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : t16;
+  attn_tree::Split split;
+  split.rows = kRows;
+  split.keys_shift = 6;
+  split.new_shift = pow2_shift(p.max_new, 3, C::kNewKeys == 64 ? 6 : 5);
+  const int page = 1 << p.page_shift, box = std::min(page, attn_tree::kMmaKeys), eb = C::FP8 ? 1 : 2;
+  CUtensorMap kc, vc, kn, vn;
+  int rc;
+  const int64_t tokens = d.T, pages = std::max<int64_t>(d.num_pages, 1);
+  // A cache without pages is never read; its map covers one row of q.
+  const void* kcp = d.num_pages ? d.k_cache : d.q;
+  const void* vcp = d.num_pages ? d.v_cache : d.q;
+  const int64_t *ks = d.k_cache_stride, *vs = d.v_cache_stride;
+  if ((rc = make_map(&kc, kcp, eb, tc, D, page, d.Hkv, pages, ks[2], ks[1], ks[0], box)) != ATTN_OK ||
+      (rc = make_map(&vc, vcp, eb, tc, D, page, d.Hkv, pages, vs[2], vs[1], vs[0], box)) != ATTN_OK ||
+      (rc = make_map(&kn, d.k_new, 2, t16, D, tokens, d.Hkv, 1, d.k_stride[0], d.k_stride[1], 0,
+                     1 << split.new_shift)) != ATTN_OK ||
+      (rc = make_map(&vn, d.v_new, 2, t16, D, tokens, d.Hkv, 1, d.v_stride[0], d.v_stride[1], 0,
+                     1 << split.new_shift)) != ATTN_OK)
+    return rc;
+  const int blocks = 2 * sms;
+  attn_tree::Scratch sc{};
+  void* base = nullptr;
+  if ((rc = tree_scratch(&sc, &base, blocks, kRows, D, s)) != ATTN_OK) return rc;
+  kern<<<blocks, attn_tree::kMmaThreads, C::kSmem, s>>>(kc, vc, kn, vn, p, split, sc, 1);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = launch_join<T, D, kRows>(p, sc, C::kShift, blocks, s);
+  cudaFreeAsync(base, s);
+  if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
+  rt_host::count_launches(2);
+  return ATTN_OK;
 }
 
 int run(const AttnTree& d, cudaStream_t s) {
@@ -401,9 +510,11 @@ int run(const AttnTree& d, cudaStream_t s) {
   using N = __nv_bfloat16;
   using E = __nv_fp8_e4m3;
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
-  if (d.dtype == ATTN_F16)
-    return fp8 ? launch_tree<H, E, 128>(p, s) : d.D == 64 ? launch_tree<H, H, 64>(p, s) : launch_tree<H, H, 128>(p, s);
-  return fp8 ? launch_tree<N, E, 128>(p, s) : d.D == 64 ? launch_tree<N, N, 64>(p, s) : launch_tree<N, N, 128>(p, s);
+  auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_mma<H, E, 128>
+                                           : d.D == 64 ? launch_tree_mma<H, H, 64> : launch_tree_mma<H, H, 128>)
+                                    : (fp8 ? launch_tree_mma<N, E, 128>
+                                           : d.D == 64 ? launch_tree_mma<N, N, 64> : launch_tree_mma<N, N, 128>);
+  return launch(d, p, dev.sms, dev.index, s);
 }
 
 template <typename Desc>
