@@ -593,18 +593,19 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
   }
 }
 
-// Joins the pieces of the items that were cut: block c takes the item whose
-// first piece block c of the first kernel ended with, if any; the pieces that
-// follow are the first ones of the blocks after it.  Added in that order, so
-// that a call gives the same bits every time.
-constexpr int kJoinThreads = 256;
+// Joins the pieces of the items that were cut: block (c, y) takes rows 16 y to
+// 16 y + 15 of the item whose first piece block c of the first kernel ended
+// with, if any; the pieces that follow are the first ones of the blocks after
+// it.  Added in that order, so that a call gives the same bits every time.
+constexpr int kJoinThreads = 256, kJoinRows = 16;
 
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ Params p,
-                                                                 const Scratch scratch, const float shift) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+    tree_join_kernel(const __grid_constant__ Params p, const Scratch scratch, const int split_rows,
+                     const int slot_rows, const float shift) {
   constexpr bool F16 = std::is_same<T, __half>::value;
-  extern __shared__ float factor[];  // [pieces][ROWS]
-  __shared__ float row_top[ROWS], row_sum[ROWS];
+  extern __shared__ float factor[];  // [pieces][16]
+  __shared__ float row_top[kJoinRows], row_sum[kJoinRows];
   __shared__ int sh_count;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -616,8 +617,11 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
     if (rec.b < 0 || rec.ends != 1) return;
   }
   const Request r = request(p, rec.b);
-  const int rows = static_cast<int>(
-      min(static_cast<int64_t>(ROWS), static_cast<int64_t>(r.count) * p.group - static_cast<int64_t>(rec.rt) * ROWS));
+  const int row0 = blockIdx.y * kJoinRows;
+  const int64_t item_rows = min(static_cast<int64_t>(split_rows),
+                                static_cast<int64_t>(r.count) * p.group - static_cast<int64_t>(rec.rt) * split_rows);
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kJoinRows), item_rows - row0));
+  if (rows <= 0) return;
   if (warp == 0) {
     int n = 0;
     for (int at = c + 1;; at += 32) {
@@ -635,17 +639,17 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   auto slot_of = [&](int i) { return i == 0 ? slot : 2 * (c + i); };
   for (int x = tid; x < n * rows; x += kJoinThreads) {
     const int i = x / rows, row = x - i * rows;
-    factor[i * ROWS + row] = scratch.m[slot_of(i) * ROWS + row];
+    factor[i * kJoinRows + row] = scratch.m[slot_of(i) * slot_rows + row0 + row];
   }
   __syncthreads();
   for (int row = warp; row < rows; row += kJoinThreads / 32) {
     float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, factor[i * ROWS + row]);
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, factor[i * kJoinRows + row]);
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     for (int i = lane; i < n; i += 32) {
-      const float f = top == -INFINITY ? 0.f : attn_sm100::ex2(factor[i * ROWS + row] - top);
-      factor[i * ROWS + row] = f;
-      sum += f * scratch.l[slot_of(i) * ROWS + row];
+      const float f = top == -INFINITY ? 0.f : attn_sm100::ex2(factor[i * kJoinRows + row] - top);
+      factor[i * kJoinRows + row] = f;
+      sum += f * scratch.l[slot_of(i) * slot_rows + row0 + row];
     }
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) row_top[row] = top, row_sum[row] = sum;
@@ -656,13 +660,13 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
-      const float f = factor[i * ROWS + row];
+      const float f = factor[i * kJoinRows + row];
       const float4 y = *reinterpret_cast<const float4*>(
-          scratch.o + (static_cast<int64_t>(slot_of(i)) * ROWS + row) * D + col);
+          scratch.o + (static_cast<int64_t>(slot_of(i)) * slot_rows + row0 + row) * D + col);
       a.x += f * y.x, a.y += f * y.y, a.z += f * y.z, a.w += f * y.w;
     }
     const float sum = row_sum[row], inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int at = rec.rt * ROWS + row;
+    const int at = rec.rt * split_rows + row0 + row;
     const int token = r.first + at / p.group, head = rec.h * p.group + at % p.group;
     *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + col) =
         make_uint2(pack2<F16>(a.x * inv, a.y * inv), pack2<F16>(a.z * inv, a.w * inv));

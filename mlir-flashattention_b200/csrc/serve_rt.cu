@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "attn_tree_mma.cuh"
+#include "attn_tree_tc.cuh"
 #include "cache_append.cuh"
 #include "cache_plan.cuh"
 #include "rotary.cuh"
@@ -357,33 +358,60 @@ int check(const AttnTree& d) {
   return ATTN_OK;
 }
 
-// 5-D tensor map of an operand seen as [pages][heads][halves][tokens][128 bytes]
-// (new tokens: one page), with a box of `box_rows` tokens of one head.
-int make_map(CUtensorMap* map, const void* base, int type_bytes, CUtensorMapDataType type, int64_t D,
-             int64_t tokens, int64_t heads, int64_t pages, int64_t s_token, int64_t s_head, int64_t s_page,
-             int box_rows) {
+// Tensor maps of 5 dimensions, innermost first, with 128-byte swizzle.
+// Strides in bytes, of dimensions 1 to 4.
+int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, const int64_t (&dims)[5],
+             int64_t (&strides)[4], const int (&box)[5]) {
   const rt_host::EncodeTiled encode = rt_host::tensor_map_encoder();
   if (!encode) return fail(ATTN_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  // Strides along an extent of one are never stepped along.
-  if (tokens == 1) s_token = D;
-  if (heads == 1) s_head = s_token * tokens;
-  if (pages == 1) s_page = s_head * heads;
-  const cuuint64_t halves = static_cast<cuuint64_t>(D * type_bytes / 128);
-  const cuuint64_t inner = 128 / type_bytes;
-  const cuuint64_t dims[5] = {inner, static_cast<cuuint64_t>(tokens), halves, static_cast<cuuint64_t>(heads),
-                              static_cast<cuuint64_t>(pages)};
-  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(s_token * type_bytes), 128,
-                                 static_cast<cuuint64_t>(s_head * type_bytes),
-                                 static_cast<cuuint64_t>(s_page * type_bytes)};
-  for (cuuint64_t s : strides)
-    if (s % 16 != 0 || s >= (1ull << 40)) return fail(ATTN_ERR_STRIDE, "a stride is negative or past 2^40 bytes");
-  const cuuint32_t box[5] = {static_cast<cuuint32_t>(inner), static_cast<cuuint32_t>(box_rows),
-                             static_cast<cuuint32_t>(halves), 1, 1};
-  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
-  const CUresult r = encode(map, type, 5, const_cast<void*>(base), dims, strides, box, step,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], step[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < 5; ++i) d[i] = static_cast<cuuint64_t>(dims[i]), b[i] = static_cast<cuuint32_t>(box[i]);
+  for (int i = 0; i < 4; ++i) {
+    if (dims[i + 1] == 1) strides[i] = 128;  // never stepped along
+    if (strides[i] < 0 || strides[i] % 16 != 0 || strides[i] >= (int64_t{1} << 40))
+      return fail(ATTN_ERR_STRIDE, "a stride is negative or past 2^40 bytes");
+    s[i] = static_cast<cuuint64_t>(strides[i]);
+  }
+  const CUresult r = encode(map, type, 5, const_cast<void*>(base), d, s, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(ATTN_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return ATTN_OK;
+}
+
+// The four key and value operands as [pages][heads][halves][tokens][128 bytes]
+// (new tokens: one page): boxes of `box` cached or `new_box` new tokens of one
+// head, all halves of its row at once or one.
+struct KeyMaps {
+  CUtensorMap kc, vc, kn, vn;
+};
+
+int make_key_maps(KeyMaps* m, const AttnTree& d, int box, int new_box, bool all_halves) {
+  const CUtensorMapDataType t16 =
+      d.dtype == ATTN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  auto one = [&](CUtensorMap* map, const void* base, CUtensorMapDataType type, int eb, int64_t tokens, int64_t pages,
+                 int64_t s_token, int64_t s_head, int64_t s_page, int rows) {
+    const int64_t inner = 128 / eb, halves = d.D * eb / 128;
+    const int64_t dims[5] = {inner, tokens, halves, d.Hkv, pages};
+    int64_t strides[4] = {s_token * eb, 128, s_head * eb, s_page * eb};
+    const int b[5] = {static_cast<int>(inner), rows, all_halves ? static_cast<int>(halves) : 1, 1, 1};
+    return make_map(map, base, type, dims, strides, b);
+  };
+  const bool fp8 = d.cache_dtype == ATTN_E4M3;
+  const CUtensorMapDataType tc = fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : t16;
+  const int eb = fp8 ? 1 : 2;
+  const int64_t *ks = d.k_cache_stride, *vs = d.v_cache_stride;
+  // A cache without pages is never read: its map stands on q.
+  const void* kc = d.num_pages ? d.k_cache : d.q;
+  const void* vc = d.num_pages ? d.v_cache : d.q;
+  const int64_t pages = std::max<int64_t>(d.num_pages, 1);
+  int rc;
+  if ((rc = one(&m->kc, kc, tc, eb, d.page_size, pages, ks[2], ks[1], ks[0], box)) != ATTN_OK ||
+      (rc = one(&m->vc, vc, tc, eb, d.page_size, pages, vs[2], vs[1], vs[0], box)) != ATTN_OK ||
+      (rc = one(&m->kn, d.k_new, t16, 2, d.T, 1, d.k_stride[0], d.k_stride[1], 0, new_box)) != ATTN_OK ||
+      (rc = one(&m->vn, d.v_new, t16, 2, d.T, 1, d.v_stride[0], d.v_stride[1], 0, new_box)) != ATTN_OK)
+    return rc;
   return ATTN_OK;
 }
 
@@ -404,20 +432,20 @@ int tree_scratch(attn_tree::Scratch* out, void** base, int blocks, int rows, int
 }
 
 // The join, launched so that it is set up while the first kernel still runs.
-template <typename T, int D, int ROWS>
-cudaError_t launch_join(const attn_tree::Params& p, const attn_tree::Scratch& sc, float shift, int blocks,
-                        cudaStream_t s) {
+template <typename T, int D>
+cudaError_t launch_join(const attn_tree::Params& p, const attn_tree::Scratch& sc, int split_rows, int slot_rows,
+                        float shift, int blocks, cudaStream_t s) {
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
+  cfg.gridDim = dim3(blocks, (split_rows + attn_tree::kJoinRows - 1) / attn_tree::kJoinRows);
   cfg.blockDim = dim3(attn_tree::kJoinThreads);
-  cfg.dynamicSmemBytes = sizeof(float) * blocks * ROWS;
+  cfg.dynamicSmemBytes = sizeof(float) * blocks * attn_tree::kJoinRows;
   cfg.stream = s;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_tree::tree_join_kernel<T, D, ROWS>, p, sc, shift);
+  return cudaLaunchKernelEx(&cfg, attn_tree::tree_join_kernel<T, D>, p, sc, split_rows, slot_rows, shift);
 }
 
 int pow2_shift(int64_t n, int lo, int hi) {
@@ -427,45 +455,80 @@ int pow2_shift(int64_t n, int lo, int hi) {
 }
 
 template <typename T, typename TC, int D>
-int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, int sms, int device, cudaStream_t s) {
+int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, const rt_host::Device& dev, cudaStream_t s) {
   using C = attn_tree::MmaCfg<T, TC, D>;
   constexpr int kRows = attn_tree::kMmaRows;
   auto kern = attn_tree::tree_mma_kernel<T, TC, D>;
   static std::once_flag once[64];
   static cudaError_t attr[64];
-  std::call_once(once[device], [&] {
-    attr[device] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
+  std::call_once(once[dev.index], [&] {
+    attr[dev.index] =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
   });
-  if (attr[device] != cudaSuccess) return cuda_fail(attr[device], "cudaFuncSetAttribute");
-  const CUtensorMapDataType t16 = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUtensorMapDataType tc = C::FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : t16;
+  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "cudaFuncSetAttribute");
   attn_tree::Split split;
   split.rows = kRows;
   split.keys_shift = 6;
   split.new_shift = pow2_shift(p.max_new, 3, C::kNewKeys == 64 ? 6 : 5);
-  const int page = 1 << p.page_shift, box = std::min(page, attn_tree::kMmaKeys), eb = C::FP8 ? 1 : 2;
-  CUtensorMap kc, vc, kn, vn;
-  int rc;
-  const int64_t tokens = d.T, pages = std::max<int64_t>(d.num_pages, 1);
-  // A cache without pages is never read; its map covers one row of q.
-  const void* kcp = d.num_pages ? d.k_cache : d.q;
-  const void* vcp = d.num_pages ? d.v_cache : d.q;
-  const int64_t *ks = d.k_cache_stride, *vs = d.v_cache_stride;
-  if ((rc = make_map(&kc, kcp, eb, tc, D, page, d.Hkv, pages, ks[2], ks[1], ks[0], box)) != ATTN_OK ||
-      (rc = make_map(&vc, vcp, eb, tc, D, page, d.Hkv, pages, vs[2], vs[1], vs[0], box)) != ATTN_OK ||
-      (rc = make_map(&kn, d.k_new, 2, t16, D, tokens, d.Hkv, 1, d.k_stride[0], d.k_stride[1], 0,
-                     1 << split.new_shift)) != ATTN_OK ||
-      (rc = make_map(&vn, d.v_new, 2, t16, D, tokens, d.Hkv, 1, d.v_stride[0], d.v_stride[1], 0,
-                     1 << split.new_shift)) != ATTN_OK)
-    return rc;
-  const int blocks = 2 * sms;
+  KeyMaps m;
+  int rc = make_key_maps(&m, d, std::min(1 << p.page_shift, attn_tree::kMmaKeys), 1 << split.new_shift, true);
+  if (rc != ATTN_OK) return rc;
+  const int blocks = 2 * dev.sms;
   attn_tree::Scratch sc{};
   void* base = nullptr;
   if ((rc = tree_scratch(&sc, &base, blocks, kRows, D, s)) != ATTN_OK) return rc;
-  kern<<<blocks, attn_tree::kMmaThreads, C::kSmem, s>>>(kc, vc, kn, vn, p, split, sc, 1);
+  kern<<<blocks, attn_tree::kMmaThreads, C::kSmem, s>>>(m.kc, m.vc, m.kn, m.vn, p, split, sc, 1);
   cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) e = launch_join<T, D, kRows>(p, sc, C::kShift, blocks, s);
+  if (e == cudaSuccess) e = launch_join<T, D>(p, sc, kRows, kRows, C::kShift, blocks, s);
+  cudaFreeAsync(base, s);
+  if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
+  rt_host::count_launches(2);
+  return ATTN_OK;
+}
+
+template <typename T, int D>
+int launch_tree_tc(const AttnTree& d, const attn_tree::Params& p, const rt_host::Device& dev, cudaStream_t s) {
+  using C = attn_tree::tc::Cfg<T, D>;
+  auto kern = attn_tree::tc::tree_tc_kernel<T, D>;
+  static std::once_flag once[64];
+  static cudaError_t attr[64];
+  static int regs[64];
+  std::call_once(once[dev.index], [&] {
+    cudaFuncAttributes fa{};
+    attr[dev.index] =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
+    if (attr[dev.index] == cudaSuccess) attr[dev.index] = cudaFuncGetAttributes(&fa, kern);
+    regs[dev.index] = fa.numRegs;
+  });
+  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "cudaFuncSetAttribute");
+  // The warpgroups' register split has to fit what a block is launched with.
+  if (regs[dev.index] * attn_tree::tc::kThreads < attn_tree::tc::kRegPool)
+    return fail(ATTN_ERR_UNSUPPORTED, "kernel built with %d registers per thread; the register split needs %d",
+                regs[dev.index], attn_tree::tc::kRegPool / attn_tree::tc::kThreads);
+  attn_tree::tc::Tiles tiles;
+  tiles.box = std::max(1, std::min(attn_tree::tc::kTileRows / p.group, p.max_new));
+  tiles.rows = tiles.box * p.group;
+  attn_tree::Split split;
+  split.rows = 2 * tiles.rows;
+  split.keys_shift = 7;
+  split.new_shift = pow2_shift(p.max_new, 3, 7);
+  KeyMaps m;
+  int rc = make_key_maps(&m, d, std::min(1 << p.page_shift, attn_tree::tc::kTileKeys), 1 << split.new_shift, false);
+  if (rc != ATTN_OK) return rc;
+  // Q as [kv heads][halves][tokens][heads of a group][128 bytes].
+  CUtensorMap mq;
+  const int64_t dims[5] = {64, p.group, d.T, D / 64, d.Hkv};
+  int64_t strides[4] = {d.q_stride[1] * 2, d.q_stride[0] * 2, 128, d.q_stride[1] * 2 * p.group};
+  const int box[5] = {64, p.group, tiles.box, 1, 1};
+  const CUtensorMapDataType t16 = C::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if ((rc = make_map(&mq, d.q, t16, dims, strides, box)) != ATTN_OK) return rc;
+  const int blocks = dev.sms;
+  attn_tree::Scratch sc{};
+  void* base = nullptr;
+  if ((rc = tree_scratch(&sc, &base, blocks, 256, D, s)) != ATTN_OK) return rc;
+  kern<<<blocks, attn_tree::tc::kThreads, C::kSmem, s>>>(mq, m.kc, m.vc, m.kn, m.vn, p, split, tiles, sc, 1);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = launch_join<T, D>(p, sc, split.rows, 256, C::kShift, blocks, s);
   cudaFreeAsync(base, s);
   if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
   rt_host::count_launches(2);
@@ -510,11 +573,16 @@ int run(const AttnTree& d, cudaStream_t s) {
   using N = __nv_bfloat16;
   using E = __nv_fp8_e4m3;
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
+  if (!fp8 && static_cast<int64_t>(p.max_new) * p.group > attn_tree::kMmaRows) {
+    auto launch = d.dtype == ATTN_F16 ? (d.D == 64 ? launch_tree_tc<H, 64> : launch_tree_tc<H, 128>)
+                                      : (d.D == 64 ? launch_tree_tc<N, 64> : launch_tree_tc<N, 128>);
+    return launch(d, p, dev, s);
+  }
   auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_mma<H, E, 128>
                                            : d.D == 64 ? launch_tree_mma<H, H, 64> : launch_tree_mma<H, H, 128>)
                                     : (fp8 ? launch_tree_mma<N, E, 128>
                                            : d.D == 64 ? launch_tree_mma<N, N, 64> : launch_tree_mma<N, N, 128>);
-  return launch(d, p, dev.sms, dev.index, s);
+  return launch(d, p, dev, s);
 }
 
 template <typename Desc>
