@@ -119,19 +119,17 @@ __device__ __forceinline__ int64_t head_units(const Params& p, const Split& s, c
 // Where a block's share begins, found by the whole block (blockDim.x threads,
 // a multiple of 32, at most 1024).
 struct Share {
-  int64_t lo, hi;  // units of this block
-  int64_t base;    // units before request b
+  int64_t lo, hi;  // units still to do
+  int64_t off;     // units of request b before lo
+  int64_t head;    // units of one of its kv-heads
   int b;           // request that holds unit lo
+  Request r;
 };
 
 __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int min_units) {
   __shared__ int64_t warp_sum[32];
-  __shared__ int64_t found_base;
-  __shared__ int found_b;
+  __shared__ Share found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  auto units = [&](int b) -> int64_t {
-    return b < p.B ? head_units(p, s, request(p, b)) * p.Hkv : 0;
-  };
   auto scan = [&](int64_t v) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -140,88 +138,91 @@ __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int
     }
     return v;
   };
+  // A thread sums requests tid, tid + threads, ..; with more requests than
+  // threads a second pass finds the one that holds the share's first unit.
   const int chunks = (p.B + blockDim.x - 1) / blockDim.x;
-  int64_t mine = 0, inc = 0;
-  for (int c = 0; c < chunks; ++c) {
-    const int64_t u = units(c * blockDim.x + tid);
-    if (chunks == 1) inc = scan(u);
-    mine += u;
+  int64_t mine = 0, head = 0;
+  Request r{};
+  for (int b = tid; b < p.B; b += blockDim.x) {
+    r = request(p, b);
+    head = head_units(p, s, r);
+    mine += head * p.Hkv;
   }
-  const int64_t sum = chunks == 1 ? inc : scan(mine);
-  if (lane == 31) warp_sum[warp] = sum;
+  int64_t inc = scan(mine);
+  if (lane == 31) warp_sum[warp] = inc;
   __syncthreads();
   int64_t total = 0, before = 0;
   for (int w = 0; w < warps; ++w) {
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
-  Share r;
   const int64_t blocks = min(static_cast<int64_t>(gridDim.x), (total + min_units - 1) / min_units);
   const int64_t c = blockIdx.x;
   if (c >= blocks) {
-    r.lo = r.hi = r.base = 0;
-    r.b = 0;
-    return r;
+    Share none{};
+    return none;
   }
-  r.lo = total * c / blocks;
-  r.hi = total * (c + 1) / blocks;
+  const int64_t lo = total * c / blocks, hi = total * (c + 1) / blocks;
+  auto offer = [&](int b, int64_t end, int64_t units) {
+    if (end - units <= lo && lo < end) found = Share{lo, hi, lo - (end - units), head, b, r};
+  };
   if (chunks == 1) {
-    const int64_t end = before + inc, start = end - mine;
-    if (start <= r.lo && r.lo < end) {
-      found_base = start;
-      found_b = tid;
-    }
+    offer(tid, before + inc, mine);
   } else {
     int64_t run = 0;
     for (int ch = 0; ch < chunks; ++ch) {
       const int b = ch * blockDim.x + tid;
-      const int64_t u = units(b), in = scan(u);
+      head = 0;
+      if (b < p.B) {
+        r = request(p, b);
+        head = head_units(p, s, r);
+      }
+      inc = scan(head * p.Hkv);
       __syncthreads();
-      if (lane == 31) warp_sum[warp] = in;
+      if (lane == 31) warp_sum[warp] = inc;
       __syncthreads();
       int64_t pre = run;
       for (int w = 0; w < warps; ++w) {
         if (w < warp) pre += warp_sum[w];
         run += warp_sum[w];
       }
-      const int64_t end = pre + in, start = end - u;
-      if (start <= r.lo && r.lo < end) {
-        found_base = start;
-        found_b = b;
-      }
+      offer(b, pre + inc, head * p.Hkv);
     }
   }
   __syncthreads();
-  r.base = found_base;
-  r.b = found_b;
-  return r;
+  return found;
 }
 
-// The next piece of a share; moves lo past it.  False at its end.
+// The next piece of a share; moves past it.  False at its end.
 __device__ __forceinline__ bool next_piece(const Params& p, const Split& s, Share& sh, Piece& out) {
   if (sh.lo >= sh.hi) return false;
-  Request r;
-  int64_t uh;
-  while (true) {
-    if (sh.b >= p.B) return false;  // lengths changed under the call
-    r = request(p, sh.b);
-    uh = head_units(p, s, r);
-    if (sh.lo - sh.base < uh * p.Hkv) break;
-    sh.base += uh * p.Hkv;
-    ++sh.b;
+  while (sh.off >= sh.head * p.Hkv) {
+    sh.off -= sh.head * p.Hkv;
+    if (++sh.b >= p.B) return false;  // lengths changed under the call
+    sh.r = request(p, sh.b);
+    sh.head = head_units(p, s, sh.r);
   }
-  int64_t off = sh.lo - sh.base;
+  const Request& r = sh.r;
+  int64_t off = sh.off;
   out.b = sh.b;
   out.r = r;
-  out.h = static_cast<int>(off / uh);
-  off -= out.h * uh;
+  out.h = 0;
+  if (off >= sh.head) {
+    out.h = (off | sh.head) >> 31 ? static_cast<int>(off / sh.head)
+                                  : static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(sh.head));
+    off -= out.h * sh.head;
+  }
   out.cached = cached_tiles(s, r);
-  if (p.mask || row_tiles(p, s, r) == 1) {
-    out.tiles = out.cached + new_tiles(p, s, r, row_tiles(p, s, r) - 1);
-    out.rt = static_cast<int>(off / out.tiles);
-    off -= static_cast<int64_t>(out.rt) * out.tiles;
+  const int rts = row_tiles(p, s, r);
+  out.rt = 0;
+  if (p.mask || rts == 1) {
+    out.tiles = out.cached + new_tiles(p, s, r, rts - 1);
+    if (rts > 1) {
+      out.rt = static_cast<int>(off / out.tiles);
+      off -= static_cast<int64_t>(out.rt) * out.tiles;
+    }
   } else {
-    for (out.rt = 0;; ++out.rt) {
+    for (;; ++out.rt) {
       out.tiles = out.cached + new_tiles(p, s, r, out.rt);
       if (off < out.tiles) break;
       off -= out.tiles;
@@ -230,6 +231,7 @@ __device__ __forceinline__ bool next_piece(const Params& p, const Split& s, Shar
   out.k0 = static_cast<int>(off);
   out.k1 = static_cast<int>(min(static_cast<int64_t>(out.tiles), off + (sh.hi - sh.lo)));
   sh.lo += out.k1 - out.k0;
+  sh.off += out.k1 - out.k0;
   return true;
 }
 
@@ -244,7 +246,7 @@ struct Scratch {
   Record* record;  // [2 blocks]
   float* m;        // [2 blocks][rows] running maximum, log2 units
   float* l;        // [2 blocks][rows]
-  float* o;        // [2 blocks][rows][D], relative to m, not divided by l
+  float4* o;       // [2 blocks][D / 4][rows], relative to m, not divided by l
 };
 
 template <typename T> __device__ __forceinline__ T from_f(float x);

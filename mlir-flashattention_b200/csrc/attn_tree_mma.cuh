@@ -116,7 +116,6 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
   using C = MmaCfg<T, TC, D>;
   constexpr bool F16 = std::is_same<T, __half>::value;
   constexpr bool FP8 = C::FP8;
-  constexpr int kHalves = D * 2 / 128;        // 128-byte column blocks of a 16-bit row
   constexpr int kSteps = D / 16;              // k-steps of Q K
   constexpr int kTilesD = D / 8;              // n-tiles of P V
   extern __shared__ uint8_t raw[];
@@ -573,7 +572,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
           uint2 w = make_uint2(pack2<F16>(x.x * inv, x.y * inv), pack2<F16>(x.z * inv, x.w * inv));
           *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + c0 + wc) = w;
         } else {
-          *reinterpret_cast<float4*>(scratch.o + (static_cast<int64_t>(slot) * kMmaRows + wr) * D + c0 + wc) = x;
+          scratch.o[(static_cast<int64_t>(slot) * (D / 4) + (c0 + wc) / 4) * kMmaRows + wr] = x;
         }
       }
       readers_sync();
@@ -655,14 +654,14 @@ __global__ void __launch_bounds__(kJoinThreads)
     if (lane == 0) row_top[row] = top, row_sum[row] = sum;
   }
   __syncthreads();
-  for (int x = tid; x < rows * (D / 4); x += kJoinThreads) {
-    const int row = x / (D / 4), col = (x - row * (D / 4)) * 4;
+  for (int x = tid; x < kJoinRows * (D / 4); x += kJoinThreads) {
+    const int row = x & (kJoinRows - 1), col = x / kJoinRows * 4;
+    if (row >= rows) continue;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
       const float f = factor[i * kJoinRows + row];
-      const float4 y = *reinterpret_cast<const float4*>(
-          scratch.o + (static_cast<int64_t>(slot_of(i)) * slot_rows + row0 + row) * D + col);
+      const float4 y = scratch.o[(static_cast<int64_t>(slot_of(i)) * (D / 4) + col / 4) * slot_rows + row0 + row];
       a.x += f * y.x, a.y += f * y.y, a.z += f * y.z, a.w += f * y.w;
     }
     const float sum = row_sum[row], inv = sum == 0.f ? 0.f : 1.f / sum;

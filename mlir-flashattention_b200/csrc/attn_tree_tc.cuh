@@ -10,7 +10,9 @@
 //   warp 9       MMA issuer (converged warp, one elected lane issues)
 //   warps 0-3    softmax of accumulator 0: one thread per query row
 //   warps 4-7    softmax of accumulator 1
-//   warps 10-11  idle (they complete warpgroup 2 for the register split)
+//   warp 10      cuts the block's share into pieces, ahead of the others, and
+//                hands them out through a short queue in shared memory
+//   warp 11      idle (it completes warpgroup 2 for the register split)
 // In the tiles at the end of the cached and of the new keys the softmax also
 // makes the value rows that do not exist 0 in shared memory: their weights are
 // 0, but what lies in memory there need not be a number.
@@ -49,11 +51,12 @@ struct Cfg {
   static constexpr int kBox = kTileKeys * 128;         // one column block of a tile
   static constexpr int kTile = kHalves * kBox;
   static constexpr int kStages = D == 128 ? 5 : 12;    // K and V tiles in the ring
-  static constexpr int kBars = 2 + 2 * kStages + 2 + 2 + 2 + 1 + 1;
-  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + kBars * 8 + 16;
+  static constexpr int kQueue = 4;                     // pieces handed out ahead
+  static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 3 + 2 * kQueue;
+  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + kBars * 8 + 16 + kQueue * 64;
   static constexpr float kShift = F16 ? 8.f : 0.f;     // weights are kept times 2^kShift
   static constexpr float kLazy = F16 ? 6.f : 8.f;      // below 2^(kShift + kLazy): 2^14 in f16
-  static_assert(kSmem <= 232448, "shared memory budget");
+  static_assert(kSmem + 512 <= 232448, "shared memory budget");
 };
 
 // Waits for this block's own copies and products in flight, abort or not.
@@ -67,46 +70,56 @@ struct Tiles {
   int box;   // tokens of a Q box
 };
 
-// How the two accumulators share a piece.
-struct Plan {
-  bool alone;
-  int end[2];  // first key tile that accumulator t does not need (of the item)
+// A piece as the block's warps need it.
+struct Job {
+  int b, h, rt;            // b = -1: no more
+  int k0, k1, cached;      // key tiles [k0, k1) of the item; tiles below `cached` are cached keys
+  int held, first, count;  // of the request
+  int alone;               // one row tile, whose key tiles both accumulators take in turn
+  int end0, end1;          // first key tile that accumulator 0 / 1 does not need
+  int rec, ends;           // scratch slot; Record::ends
+  int rows;                // query rows of the item
 
-  // Accumulator t takes key tile k of a piece that begins at k0.
-  __device__ __forceinline__ bool takes(int t, int k, int k0) const {
-    return alone ? ((k - k0) & 1) == t : k < end[t];
+  // Accumulator t takes key tile k.
+  __device__ __forceinline__ bool takes(int t, int k) const {
+    return alone ? ((k - k0) & 1) == t : k < (t ? end1 : end0);
   }
-  __device__ __forceinline__ int first(int t, int k0) const { return alone ? k0 + t : k0; }
+  __device__ __forceinline__ int from(int t) const { return alone ? k0 + t : k0; }
   __device__ __forceinline__ int step() const { return alone ? 2 : 1; }
-  // End of accumulator t's tiles in a piece that ends at k1.
-  __device__ __forceinline__ int stop(int t, int k1) const { return min(end[t], k1); }
-};
-
-__device__ __forceinline__ Plan make_plan(const Params& p, const Split& s, const Tiles& tl, const Piece& pc) {
-  Plan r;
-  const int64_t rows = static_cast<int64_t>(pc.r.count) * p.group - static_cast<int64_t>(pc.rt) * s.rows;
-  r.alone = rows <= tl.rows;
-  r.end[0] = r.end[1] = pc.tiles;
-  if (!r.alone && p.mask == nullptr) {
-    const int keys = min(pc.r.count, (pc.rt * s.rows + tl.rows - 1) / p.group + 1);
-    r.end[0] = pc.cached + ((keys + (1 << s.new_shift) - 1) >> s.new_shift);
+  __device__ __forceinline__ int stop(int t) const { return min(t ? end1 : end0, k1); }
+  // Keys that exist in tile k.
+  __device__ __forceinline__ int here(const Split& s, int k) const {
+    return k < cached ? min(kTileKeys, held - (k << s.keys_shift))
+                      : min(1 << s.new_shift, count - ((k - cached) << s.new_shift));
   }
-  return r;
-}
+};
+static_assert(sizeof(Job) <= 64, "a queue entry");
 
-// Keys that exist in tile k of a piece.
-__device__ __forceinline__ int keys_here(const Split& s, const Piece& pc, int k) {
-  return k < pc.cached ? min(kTileKeys, pc.r.held - (k << s.keys_shift))
-                       : min(1 << s.new_shift, pc.r.count - ((k - pc.cached) << s.new_shift));
+__device__ __forceinline__ Job make_job(const Params& p, const Split& s, const Tiles& tl, const Piece& pc, int rec) {
+  Job j;
+  j.b = pc.b, j.h = pc.h, j.rt = pc.rt;
+  j.k0 = pc.k0, j.k1 = pc.k1, j.cached = pc.cached;
+  j.held = pc.r.held, j.first = pc.r.first, j.count = pc.r.count;
+  j.rows = static_cast<int>(min(static_cast<int64_t>(s.rows), static_cast<int64_t>(pc.r.count) * p.group -
+                                                                   static_cast<int64_t>(pc.rt) * s.rows));
+  j.alone = j.rows <= tl.rows;
+  j.end0 = j.end1 = pc.tiles;
+  if (!j.alone && p.mask == nullptr) {
+    const int keys = min(pc.r.count, (pc.rt * s.rows + tl.rows - 1) / p.group + 1);
+    j.end0 = pc.cached + ((keys + (1 << s.new_shift) - 1) >> s.new_shift);
+  }
+  j.rec = rec;
+  j.ends = (pc.k0 == 0 ? 1 : 0) | (pc.k1 == pc.tiles ? 2 : 0);
+  return j;
 }
 
 // Bits of one row of the mask for keys [first, first + here) of its request's
 // new ones: the warp reads each row of its 32 query rows' tokens together.
-__device__ __forceinline__ void mask_bits(const Params& p, const Piece& pc, int token, int t_lo, int t_hi,
-                                          int first, int here, int lane, uint32_t (&bits)[4]) {
+__device__ __forceinline__ void mask_bits(const Params& p, int row0, int token, int t_lo, int t_hi, int first,
+                                          int here, int lane, uint32_t (&bits)[4]) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) bits[w] = 0xffffffffu;
-  const uint8_t* const m = p.mask + static_cast<int64_t>(pc.r.first) * p.mask_stride + first;
+  const uint8_t* const m = p.mask + static_cast<int64_t>(row0) * p.mask_stride + first;
   for (int t0 = t_lo; t0 <= t_hi; t0 += 4) {
     uint32_t b[4][4];
 #pragma unroll
@@ -145,12 +158,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* const kv_full = bars + 2;
   uint64_t* const kv_empty = kv_full + C::kStages;
   uint64_t* const s_full = kv_empty + C::kStages;
-  uint64_t* const p_ready = s_full + 2;
-  uint64_t* const pv_done = p_ready + 2;
-  uint64_t* const o_free = pv_done + 2;  // both accumulators of a piece have been read
-  uint64_t* const drain = o_free + 1;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* const p_ready = s_full + 2;    // [half of P][accumulator]
+  uint64_t* const pv_done = p_ready + 4;
+  uint64_t* const o_free = pv_done + 2;    // both accumulators of a piece have been read
+  uint64_t* const met = o_free + 1;        // alone: both groups are at one point
+  uint64_t* const drain = met + 1;
+  uint64_t* const job_full = drain + 1;
+  uint64_t* const job_empty = job_full + C::kQueue;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(job_empty + C::kQueue);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  Job* const jobs = reinterpret_cast<Job*>(tmem_slot + 4);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -164,10 +181,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_ready[t], 4);
+      mbar_init(&p_ready[2 + t], 4);
       mbar_init(&pv_done[t], 1);
     }
     mbar_init(o_free, 256);
+    mbar_init(met, 256);
     mbar_init(drain, 1);
+    for (int i = 0; i < C::kQueue; ++i) {
+      mbar_init(&job_full[i], 1);
+      mbar_init(&job_empty[i], 10);  // producer, issuer and eight softmax warps
+    }
     *abort_flag = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -182,52 +205,57 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int64_t share_lo = share.lo;
-  Piece pc;
   auto slot = [](int pos) { return pos % C::kStages; };
   auto par = [](int pos) { return static_cast<uint32_t>((pos / C::kStages) & 1); };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, p.status, kWaitLimitNs));
+  };
+  // The n-th piece; false when there is none (or the block gives up).
+  auto take_job = [&](int n, Job& j) {
+    const int i = n % C::kQueue;
+    if (!wait(&job_full[i], static_cast<uint32_t>((n / C::kQueue) & 1))) return false;
+    j = jobs[i];
+    return j.b >= 0;
+  };
+  auto leave_job = [&](int n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&job_empty[n % C::kQueue]);
   };
 
   if (warp >= 8) {
     setmaxnreg_dec<kRegsOther>();
     if (warp == 8) {
       // ---------------------------------------------------------- producer
-      if (lane == 0) {
-        prefetch_tmap(&map_q);
-        prefetch_tmap(&map_kc);
-        prefetch_tmap(&map_vc);
-        prefetch_tmap(&map_kn);
-        prefetch_tmap(&map_vn);
-      }
       const int seg_shift = min(p.page_shift, split.keys_shift);  // rows of a page segment, log2
-      int pos = 0, qi = 0;
+      int pos = 0, n = 0;
       bool ok = true;
-      while (ok && next_piece(p, split, share, pc)) {
-        const Plan plan = make_plan(p, split, tiles, pc);
-        const int32_t* const row = p.table + pc.b * p.table_stride;
-        for (int k = pc.k0; k < pc.k1 && ok; ++k) {
-          const bool cached = k < pc.cached;
-          const int first = cached ? k << split.keys_shift : (k - pc.cached) << split.new_shift;
-          int segs = 1, page = 0, at = 0;
-          if (cached) {
-            segs = (keys_here(split, pc, k) + (1 << seg_shift) - 1) >> seg_shift;
-            if (lane < segs) {
-              const int key = first + (lane << seg_shift);
-              page = __ldg(row + (key >> p.page_shift));
-              at = key & ((1 << p.page_shift) - 1);
-              if (page < 0 || page >= p.num_pages) {
-                atomicCAS(p.status, 0, ATTN_ERR_INVALID);
-                page = max(p.num_pages, 1);  // outside the map: zeros
-              }
+      Job j;
+      for (; ok && take_job(n, j); ++n) {
+        leave_job(n);
+        const int32_t* const row = p.table + j.b * p.table_stride;
+        auto segments = [&](int k) { return (j.here(split, k) + (1 << seg_shift) - 1) >> seg_shift; };
+        auto page_of = [&](int k) {  // of this lane's segment
+          if (k >= min(j.cached, j.k1) || lane >= segments(k)) return 0;
+          return __ldg(row + (((k << split.keys_shift) + (lane << seg_shift)) >> p.page_shift));
+        };
+        int page_next = page_of(j.k0);
+        for (int k = j.k0; k < j.k1 && ok; ++k) {
+          const bool cached = k < j.cached;
+          const int segs = cached ? segments(k) : 1;
+          int page = page_next, at = 0;
+          page_next = page_of(k + 1);  // a tile ahead of its use
+          if (cached && lane < segs) {
+            at = ((k << split.keys_shift) + (lane << seg_shift)) & ((1 << p.page_shift) - 1);
+            if (page < 0 || page >= p.num_pages) {
+              atomicCAS(p.status, 0, ATTN_ERR_INVALID);
+              page = max(p.num_pages, 1);  // outside the map: zeros
             }
           }
-          for (int v = 0; v < 2 && ok; ++v, ++pos) {
+          for (int v = 0; v < 2; ++v, ++pos) {
             const int s = slot(pos);
             ok = wait(&kv_empty[s], par(pos) ^ 1u);
             if (!ok) break;
-            const int seg = cached ? 128 << seg_shift : 128 << split.new_shift;
+            const int seg = 128 << (cached ? seg_shift : split.new_shift);
             if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], segs * seg * C::kHalves);
             __syncwarp();
             if (lane < segs) {
@@ -235,33 +263,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int c = 0; c < C::kHalves; ++c) {
                 if (cached)
-                  tma_load_5d(dst + c * C::kBox, v ? &map_vc : &map_kc, &kv_full[s], 0, at, c, pc.h, page);
+                  tma_load_5d(dst + c * C::kBox, v ? &map_vc : &map_kc, &kv_full[s], 0, at, c, j.h, page);
                 else
-                  tma_load_5d(dst + c * C::kBox, v ? &map_vn : &map_kn, &kv_full[s], 0, pc.r.first + first, c, pc.h, 0);
+                  tma_load_5d(dst + c * C::kBox, v ? &map_vn : &map_kn, &kv_full[s], 0,
+                              j.first + ((k - j.cached) << split.new_shift), c, j.h, 0);
               }
             }
           }
-          if (k == pc.k0 && ok) {
-            // Q behind the piece's first keys, which need no wait for the
+          if (k == j.k0 && ok) {
+            // Q behind the piece's first keys, which need not wait for the
             // last S product of the piece before.
-            ok = wait(q_empty, static_cast<uint32_t>(qi & 1) ^ 1u);
+            ok = wait(q_empty, static_cast<uint32_t>(n & 1) ^ 1u);
             if (!ok) break;
             if (lane == 0) {
-              const int n = plan.alone ? 1 : 2;
-              mbar_arrive_expect_tx(q_full, n * C::kHalves * tiles.rows * 128);
-              for (int t = 0; t < n; ++t)
+              const int m = j.alone ? 1 : 2;
+              mbar_arrive_expect_tx(q_full, m * C::kHalves * tiles.rows * 128);
+              for (int t = 0; t < m; ++t)
                 for (int c = 0; c < C::kHalves; ++c)
                   tma_load_5d(smem_u32(sQ + t * C::kTile + c * C::kBox), &map_q, q_full, 0, 0,
-                              pc.r.first + pc.rt * (2 * tiles.box) + t * tiles.box, c, pc.h);
+                              j.first + j.rt * (2 * tiles.box) + t * tiles.box, c, j.h);
             }
-            ++qi;
             __syncwarp();
           }
         }
       }
-      // Every copy that was started lands before the block may end.
+      // Every copy that was started lands before the block may end.  (n counts
+      // the pieces whose Q was asked for; after a wait that gave up, q_full may
+      // be one phase behind, which this wait then also gives up on.)
       if (lane == 0) {
-        if (qi > 0) drain_wait(q_full, static_cast<uint32_t>((qi - 1) & 1), p.status);
+        if (n > 0) drain_wait(q_full, static_cast<uint32_t>((n - 1) & 1), p.status);
         for (int s = 0; s < C::kStages && s < pos; ++s)
           drain_wait(&kv_full[s], static_cast<uint32_t>(((pos - 1 - s) / C::kStages) & 1), p.status);
       }
@@ -275,18 +305,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t dK0 = make_sdesc(smem_u32(sKV), 16, 1024);
       const uint64_t dV0 = make_sdesc(smem_u32(sKV), C::kBox, 1024);
       const uint32_t lead = elect_one();
-      int base = 0, qi = 0;
-      int s_cnt[2] = {0, 0}, pv_cnt[2] = {0, 0}, items = 0;
+      int base = 0, n = 0;
+      int pv_cnt[2] = {0, 0};
       bool ok = true;
-      while (ok && next_piece(p, split, share, pc)) {
-        const Plan plan = make_plan(p, split, tiles, pc);
-        auto kpos = [&](int k) { return base + 2 * (k - pc.k0); };
+      Job j;
+      for (; ok && take_job(n, j); ++n) {
+        leave_job(n);
+        auto kpos = [&](int k) { return base + 2 * (k - j.k0); };
         int left = 0;  // S products still to issue from this Q
         for (int t = 0; t < 2; ++t) {
-          const int f = plan.first(t, pc.k0), e = plan.stop(t, pc.k1);
-          if (f < e) left += (e - f + plan.step() - 1) / plan.step();
+          const int f = j.from(t), e = j.stop(t);
+          if (f < e) left += (e - f + j.step() - 1) / j.step();
         }
-        int k_seen = pc.k0 - 1;  // last key tile whose K has arrived
+        int k_seen = j.k0 - 1;  // last key tile whose K has arrived
         auto issue_S = [&](int t, int k) {
           if (k > k_seen) {
             if (!wait(&kv_full[slot(kpos(k))], par(kpos(k)))) return false;
@@ -297,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // accumulator and so are not ordered by their issue.
           if (pv_cnt[t] > 0 && !wait(&pv_done[t], static_cast<uint32_t>((pv_cnt[t] - 1) & 1))) return false;
           tc_fence_after();
-          const uint64_t a0 = dQ0 + static_cast<uint64_t>(((plan.alone ? 0 : t) * C::kTile) >> 4);
+          const uint64_t a0 = dQ0 + static_cast<uint64_t>(((j.alone ? 0 : t) * C::kTile) >> 4);
           const uint64_t b0 = dK0 + static_cast<uint64_t>((slot(kpos(k)) * C::kTile) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
@@ -305,49 +336,74 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma_ss_lead<0>(lead, tmem + t * 128, a0 + (off >> 4), b0 + (off >> 4), idS, kk > 0 ? 1u : 0u);
           }
           mma_commit_lead(lead, &s_full[t]);
-          ++s_cnt[t];
           // K is free after its last S product (accumulator 1's, of two).
-          if (plan.alone || t == 1) mma_commit_lead(lead, &kv_empty[slot(kpos(k))]);
+          if (j.alone || t == 1) mma_commit_lead(lead, &kv_empty[slot(kpos(k))]);
           if (--left == 0) mma_commit_lead(lead, q_empty);
           return true;
         };
-        ok = wait(q_full, static_cast<uint32_t>(qi & 1));
-        for (int t = 0; t < 2 && ok; ++t) {
-          const int f = plan.first(t, pc.k0);
-          if (f < plan.stop(t, pc.k1)) ok = issue_S(t, f);
-        }
-        bool first_pv[2] = {true, true}, waited = items == 0;
-        for (int k = pc.k0; k < pc.k1 && ok; ++k) {
+        ok = wait(q_full, static_cast<uint32_t>(n & 1));
+        for (int t = 0; t < 2 && ok; ++t)
+          if (j.from(t) < j.stop(t)) ok = issue_S(t, j.from(t));
+        bool first_pv[2] = {true, true}, waited = n == 0;
+        for (int k = j.k0; k < j.k1 && ok; ++k) {
           const int vp = kpos(k) + 1;
           ok = wait(&kv_full[slot(vp)], par(vp));
           for (int t = 0; t < 2 && ok; ++t) {
-            if (!plan.takes(t, k, pc.k0)) continue;
+            if (!j.takes(t, k)) continue;
             ok = wait(&p_ready[t], static_cast<uint32_t>(pv_cnt[t] & 1));
             if (ok && !waited) {  // O of the piece before has been read
-              ok = wait(o_free, static_cast<uint32_t>((items - 1) & 1));
+              ok = wait(o_free, static_cast<uint32_t>((n - 1) & 1));
               waited = true;
             }
             if (!ok) break;
             tc_fence_after();
             const uint64_t b0 = dV0 + static_cast<uint64_t>((slot(vp) * C::kTile) >> 4);
+            // P V of keys 0-63 while the softmax stores the weights of 64-127.
 #pragma unroll
-            for (int kk = 0; kk < kTileKeys / 16; ++kk)
-              mma_ts_lead<0>(lead, tmem + 256 + t * D, tmem + t * 128 + kk * 8,
-                             b0 + static_cast<uint64_t>((kk * 16 * 128) >> 4), idO, (!first_pv[t] || kk > 0) ? 1u : 0u);
+            for (int h = 0; h < 2; ++h) {
+              if (h == 1) {
+                ok = wait(&p_ready[2 + t], static_cast<uint32_t>(pv_cnt[t] & 1));
+                if (!ok) break;
+                tc_fence_after();
+              }
+#pragma unroll
+              for (int kk = h * (kTileKeys / 32); kk < (h + 1) * (kTileKeys / 32); ++kk)
+                mma_ts_lead<0>(lead, tmem + 256 + t * D, tmem + t * 128 + kk * 8,
+                               b0 + static_cast<uint64_t>((kk * 16 * 128) >> 4), idO,
+                               (!first_pv[t] || kk > 0) ? 1u : 0u);
+            }
+            if (!ok) break;
             first_pv[t] = false;
             mma_commit_lead(lead, &pv_done[t]);
             ++pv_cnt[t];
-            const int next = k + plan.step();
-            if (next < plan.stop(t, pc.k1)) ok = issue_S(t, next);
+            const int next = k + j.step();
+            if (next < j.stop(t)) ok = issue_S(t, next);
           }
           if (ok) mma_commit_lead(lead, &kv_empty[slot(vp)]);  // V free after its P V products
         }
-        base += 2 * (pc.k1 - pc.k0);
-        ++qi;
-        ++items;
+        base += 2 * (j.k1 - j.k0);
       }
       mma_commit_lead(lead, drain);
       if (lane == 0) drain_wait(drain, 0, p.status);
+      __syncwarp();
+    } else if (warp == 10) {
+      // ---------------------------------------------------------- pieces
+      const int64_t share_lo = share.lo;
+      Piece pc;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int i = n % C::kQueue;
+        const int64_t lo = share.lo;
+        const bool more = next_piece(p, split, share, pc);
+        ok = wait(&job_empty[i], static_cast<uint32_t>((n / C::kQueue) & 1) ^ 1u);
+        if (!ok) break;
+        if (lane == 0) {
+          if (more) jobs[i] = make_job(p, split, tiles, pc, 2 * blockIdx.x + (lo == share_lo ? 0 : 1));
+          else jobs[i].b = -1;
+          mbar_arrive(&job_full[i]);
+        }
+        if (!more) break;
+      }
       __syncwarp();
     }
   } else {
@@ -363,45 +419,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float hidden = pos ? -INFINITY : INFINITY;
     int steps = 0;  // S tiles of this accumulator so far
     int base = 0;   // ring position of the piece's first K
+    int meets = 0;  // phases of `met` so far
     bool ok = true;
-    while (next_piece(p, split, share, pc)) {
-      const Plan plan = make_plan(p, split, tiles, pc);
-      const int64_t item_rows = static_cast<int64_t>(pc.r.count) * p.group - static_cast<int64_t>(pc.rt) * split.rows;
-      const int row0 = plan.alone ? 0 : t * tiles.rows;             // of the item
-      const int rows = static_cast<int>(min(static_cast<int64_t>(tiles.rows), item_rows - row0));
-      const int at = pc.rt * split.rows + row0 + min(r, max(rows, 1) - 1);
-      const int token = at / p.group, head = pc.h * p.group + at % p.group;
+    Job j;
+    for (int n = 0; ok && take_job(n, j); ++n) {
+      leave_job(n);
+      const int row0 = j.alone ? 0 : t * tiles.rows;  // of the item
+      const int rows = min(tiles.rows, j.rows - row0);
+      const int at = j.rt * split.rows + row0 + min(r, max(rows, 1) - 1);
+      const int token = at / p.group;
       const bool busy = (warp & 3) * 32 < rows;  // a warp without rows only keeps step
       float m = -INFINITY, l = 0.f;
-      bool first = true;
-      const int stop = plan.stop(t, pc.k1);
-      // Mask bits of the first new tile, read while its keys are on their way.
-      uint32_t bits[4] = {0, 0, 0, 0};
-      const int t_lo = __shfl_sync(0xffffffffu, token, 0), t_hi = __shfl_sync(0xffffffffu, token, 31);
-      int bits_of = -1;
-      if (p.mask && busy && stop > pc.cached) {
-        const int f = plan.first(t, pc.k0);
-        const int k = max(pc.cached, f) + (plan.alone && pc.cached > f ? ((pc.cached - f) & 1) : 0);
-        if (k < stop) {
-          mask_bits(p, pc, token, t_lo, t_hi, (k - pc.cached) << split.new_shift, keys_here(split, pc, k), lane, bits);
-          bits_of = k;
-        }
-      }
-      for (int k = plan.first(t, pc.k0); k < stop; k += plan.step(), ++steps) {
-        const bool cached = k < pc.cached;
-        const int here = keys_here(split, pc, k);
-        if (!cached && p.mask && busy && bits_of != k) {
-          mask_bits(p, pc, token, t_lo, t_hi, (k - pc.cached) << split.new_shift, here, lane, bits);
-          bits_of = k;
-        }
-        if (ok) ok = wait(&s_full[t], static_cast<uint32_t>(steps & 1));
+      const int from = j.from(t), stop = j.stop(t);
+      for (int k = from; k < stop && ok; k += j.step(), ++steps) {
+        const bool cached = k < j.cached;
+        const int here = j.here(split, k);
+        uint32_t bits[4];
+        const bool masked = !cached && p.mask != nullptr && busy;
+        if (masked)
+          mask_bits(p, j.first, token, __shfl_sync(0xffffffffu, token, 0), __shfl_sync(0xffffffffu, token, 31),
+                    (k - j.cached) << split.new_shift, here, lane, bits);
+        ok = wait(&s_full[t], static_cast<uint32_t>(steps & 1));
+        if (!ok) break;
         tc_fence_after();
-        if (here < kTileKeys && (t == 0 || !plan.takes(0, k, pc.k0))) {
+        if (here < kTileKeys && (t == 0 || !j.takes(0, k))) {
           // Accumulator 0's products of a tile come first.  The tile before in
           // V's slot has been used (S of this one is complete), so the phase
           // waited for is the slot's next.
-          const int vp = base + 2 * (k - pc.k0) + 1;
-          if (ok) ok = wait(&kv_full[slot(vp)], par(vp));
+          const int vp = base + 2 * (k - j.k0) + 1;
+          ok = wait(&kv_full[slot(vp)], par(vp));
+          if (!ok) break;
           if (r >= here) {
             uint8_t* const v = sKV + slot(vp) * C::kTile + r * 128;
 #pragma unroll
@@ -411,32 +458,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_proxy_async_smem();
         }
+        float s[128];
         if (busy) {
-          float s[128];
-          {
-            uint32_t r0[32], r1[32], r2[32], r3[32];
-            tmem_ld32(tS + 0, r0);
-            tmem_ld32(tS + 32, r1);
-            tmem_ld32(tS + 64, r2);
-            tmem_ld32(tS + 96, r3);
-            tmem_wait_ld();
+          uint32_t r0[32], r1[32], r2[32], r3[32];
+          tmem_ld32(tS + 0, r0);
+          tmem_ld32(tS + 32, r1);
+          tmem_ld32(tS + 64, r2);
+          tmem_ld32(tS + 96, r3);
+          tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              s[i] = __uint_as_float(r0[i]);
-              s[32 + i] = __uint_as_float(r1[i]);
-              s[64 + i] = __uint_as_float(r2[i]);
-              s[96 + i] = __uint_as_float(r3[i]);
-            }
+          for (int i = 0; i < 32; ++i) {
+            s[i] = __uint_as_float(r0[i]);
+            s[32 + i] = __uint_as_float(r1[i]);
+            s[64 + i] = __uint_as_float(r2[i]);
+            s[96 + i] = __uint_as_float(r3[i]);
           }
           int lim = here;  // keys below it are seen
-          if (!cached) {
-            if (p.mask) {
+          if (masked) {
 #pragma unroll
-              for (int c = 0; c < 128; ++c)
-                if ((bits[c >> 5] >> (c & 31)) & 1u) s[c] = hidden;
-            } else {
-              lim = min(here, token - ((k - pc.cached) << split.new_shift) + 1);
-            }
+            for (int c = 0; c < 128; ++c)
+              if ((bits[c >> 5] >> (c & 31)) & 1u) s[c] = hidden;
+          } else if (!cached) {
+            lim = min(here, token - ((k - j.cached) << split.new_shift) + 1);
           }
           if (__any_sync(0xffffffffu, lim < 128)) {
 #pragma unroll
@@ -467,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             alpha = ex2(m - top);
             m = top;
           }
-          if (__any_sync(0xffffffffu, !first && alpha != 1.f)) {
+          if (__any_sync(0xffffffffu, k != from && alpha != 1.f)) {
             // The P V product before this S product is complete (see issue_S).
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -479,12 +522,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32(tO + c * 32, o);
             }
           }
-          first = false;
-          const float sub = m == -INFINITY ? 0.f : C::kShift - m;
-          const uint64_t sl2x2 = f2_pack(sl2, sl2), subx2 = f2_pack(sub, sub);
-          uint64_t sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
+          l *= alpha;
+        }
+        // Weights in two halves, each published as it is stored.
+        const float sub = m == -INFINITY ? 0.f : C::kShift - m;
+        const uint64_t sl2x2 = f2_pack(sl2, sl2), subx2 = f2_pack(sub, sub);
+        uint64_t sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
+          if (busy) {
             uint32_t pk[32];
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
@@ -497,103 +543,95 @@ __global__ void __launch_bounds__(kThreads, 1)
               pk[c] = pack2<F16>(e0, e1);
             }
             tmem_st32(tS + 32 * h, pk);
+            tmem_wait_st();
           }
-          float q0, q1;
-          f2_unpack(f2_add(sum0, sum1), q0, q1);
-          l = l * alpha + (q0 + q1);
-          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * h + t]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[t]);
+        float q0, q1;
+        f2_unpack(f2_add(sum0, sum1), q0, q1);
+        l += q0 + q1;
       }
-      base += 2 * (pc.k1 - pc.k0);
+      if (!ok) break;
+      base += 2 * (j.k1 - j.k0);
       // ------------------------------------------------------------ a piece ends
-      const bool has = plan.first(t, pc.k0) < stop;
-      if (has && ok) ok = wait(&pv_done[t], static_cast<uint32_t>((steps - 1) & 1));
+      const bool has = from < stop, whole = j.ends == 3;
+      if (has && !wait(&pv_done[t], static_cast<uint32_t>((steps - 1) & 1))) break;
       tc_fence_after();
-      const bool whole = pc.k0 == 0 && pc.k1 == pc.tiles;
-      const int rec = 2 * blockIdx.x + (share.lo - (pc.k1 - pc.k0) == share_lo ? 0 : 1);
       // Alone: columns [D/2 t, D/2 t + D/2) of both accumulators; else all of its own.
       float f0 = 1.f, f1 = 0.f, mm = m, ll = l;
-      bool has0 = has, has1 = false;
-      if (plan.alone) {
+      if (j.alone) {
         // Both groups' maxima and sums meet in this piece's scratch slot (shared
         // memory is full).
-        scratch.m[rec * 256 + t * 128 + r] = m;
-        scratch.l[rec * 256 + t * 128 + r] = l;
+        scratch.m[j.rec * 256 + t * 128 + r] = m;
+        scratch.l[j.rec * 256 + t * 128 + r] = l;
         __threadfence();  // read past L1
         tc_fence_before();
-        __syncwarp();
-        asm volatile("barrier.sync 2, 256;" ::: "memory");
+        mbar_arrive(met);
+        if (!wait(met, static_cast<uint32_t>(meets++ & 1))) break;
         tc_fence_after();
-        has0 = true, has1 = pc.k1 - pc.k0 > 1;
-        const float m0 = __ldcg(scratch.m + rec * 256 + r), m1 = __ldcg(scratch.m + rec * 256 + 128 + r);
+        const float m0 = __ldcg(scratch.m + j.rec * 256 + r), m1 = __ldcg(scratch.m + j.rec * 256 + 128 + r);
         mm = fmaxf(m0, m1);
         f0 = mm == -INFINITY ? 0.f : ex2(m0 - mm);
         f1 = mm == -INFINITY ? 0.f : ex2(m1 - mm);
-        ll = f0 * __ldcg(scratch.l + rec * 256 + r) + f1 * __ldcg(scratch.l + rec * 256 + 128 + r);
+        ll = f0 * __ldcg(scratch.l + j.rec * 256 + r) + f1 * __ldcg(scratch.l + j.rec * 256 + 128 + r);
+        mbar_arrive(met);  // both groups have read the slot
+        if (!wait(met, static_cast<uint32_t>(meets++ & 1))) break;
       }
-      const bool live = r < rows && busy;
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      const bool live = r < rows;
       const bool none = ll == 0.f;  // nothing seen: 0 whatever the accumulator holds
-      const float w0 = whole ? f0 * inv : f0, w1 = whole ? f1 * inv : f1;
-      T* const orow = static_cast<T*>(p.o) + static_cast<int64_t>(pc.r.first + token) * p.o_st + head * p.o_sh;
-      float* const srow = scratch.o + (static_cast<int64_t>(rec) * 256 + row0 + r) * D;
-      const uint32_t tA = tmem + lane_off + 256 + (plan.alone ? 0 : t * D), tB = tmem + lane_off + 256 + D;
-      const int c_lo = plan.alone ? t * (D / 2) : 0, c_hi = plan.alone ? c_lo + D / 2 : D;
+      const float inv = whole && !none ? 1.f / ll : 1.f;
+      const float w0 = f0 * inv, w1 = f1 * inv;
+      const int head = j.h * p.group + at % p.group;
+      T* const orow = static_cast<T*>(p.o) + static_cast<int64_t>(j.first + token) * p.o_st + head * p.o_sh;
+      float4* const srow = scratch.o + static_cast<int64_t>(j.rec) * (D / 4) * 256 + row0 + r;
+      const uint32_t tA = j.alone ? tmem + lane_off + 256 : tO;
+      const bool two = j.alone && j.k1 - j.k0 > 1, any = j.alone || has;
+      const int c_lo = j.alone ? t * (D / 2) : 0, c_hi = j.alone ? c_lo + D / 2 : D;
       if (busy) {
         for (int c = c_lo; c < c_hi; c += 32) {
           uint32_t a[32];
-          if (has0) {
-            tmem_ld32(tA + c, a);
-            tmem_wait_ld();
-          }
+          tmem_ld32(tA + c, a);
+          tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            a[i] = has0 && !none ? __float_as_uint(__uint_as_float(a[i]) * w0) : 0u;
-          if (has1 && plan.alone) {
+          for (int i = 0; i < 32; ++i) a[i] = any && !none ? __float_as_uint(__uint_as_float(a[i]) * w0) : 0u;
+          if (two) {
             uint32_t b[32];
-            tmem_ld32(tB + c, b);
+            tmem_ld32(tA + D + c, b);
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!none) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), w1, __uint_as_float(a[i])));
           }
-          if (live) {
-            if (whole) {
+          if (live && whole) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                reinterpret_cast<uint4*>(orow + c)[i] =
-                    make_uint4(pack2<F16>(__uint_as_float(a[8 * i]), __uint_as_float(a[8 * i + 1])),
-                               pack2<F16>(__uint_as_float(a[8 * i + 2]), __uint_as_float(a[8 * i + 3])),
-                               pack2<F16>(__uint_as_float(a[8 * i + 4]), __uint_as_float(a[8 * i + 5])),
-                               pack2<F16>(__uint_as_float(a[8 * i + 6]), __uint_as_float(a[8 * i + 7])));
-            } else {
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4*>(orow + c)[i] =
+                  make_uint4(pack2<F16>(__uint_as_float(a[8 * i]), __uint_as_float(a[8 * i + 1])),
+                             pack2<F16>(__uint_as_float(a[8 * i + 2]), __uint_as_float(a[8 * i + 3])),
+                             pack2<F16>(__uint_as_float(a[8 * i + 4]), __uint_as_float(a[8 * i + 5])),
+                             pack2<F16>(__uint_as_float(a[8 * i + 6]), __uint_as_float(a[8 * i + 7])));
+          } else if (live) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                reinterpret_cast<uint4*>(srow + c)[i] = make_uint4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
-            }
+            for (int i = 0; i < 8; ++i)
+              srow[(c / 4 + i) * 256] = make_float4(__uint_as_float(a[4 * i]), __uint_as_float(a[4 * i + 1]),
+                                                    __uint_as_float(a[4 * i + 2]), __uint_as_float(a[4 * i + 3]));
           }
         }
       }
       tc_fence_before();
       mbar_arrive(o_free);
-      if (plan.alone) {  // both groups have read the slot
-        __syncwarp();
-        asm volatile("barrier.sync 2, 256;" ::: "memory");
-      }
-      if (live && (!plan.alone || t == 0)) {
+      if (live && (!j.alone || t == 0)) {
         if (!whole) {
-          scratch.m[rec * 256 + row0 + r] = mm;
-          scratch.l[rec * 256 + row0 + r] = ll;
+          scratch.m[j.rec * 256 + row0 + r] = mm;
+          scratch.l[j.rec * 256 + row0 + r] = ll;
         } else if (p.lse) {
-          p.lse[static_cast<int64_t>(pc.r.first + token) * p.Hq + head] =
-              ll == 0.f ? -INFINITY : (mm - C::kShift + log2f(ll)) * kLn2;
+          p.lse[static_cast<int64_t>(j.first + token) * p.Hq + head] =
+              none ? -INFINITY : (mm - C::kShift + log2f(ll)) * kLn2;
         }
       }
-      if (!whole && tid == 0)
-        scratch.record[rec] = Record{pc.b, pc.h, pc.rt, (pc.k0 == 0 ? 1 : 0) | (pc.k1 == pc.tiles ? 2 : 0)};
+      if (!whole && tid == 0) scratch.record[j.rec] = Record{j.b, j.h, j.rt, j.ends};
     }
   }
   tc_fence_before();

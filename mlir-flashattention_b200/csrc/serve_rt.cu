@@ -427,7 +427,7 @@ int tree_scratch(attn_tree::Scratch* out, void** base, int blocks, int rows, int
   out->record = reinterpret_cast<attn_tree::Record*>(at);
   out->m = reinterpret_cast<float*>(at + rec);
   out->l = reinterpret_cast<float*>(at + rec + ml);
-  out->o = reinterpret_cast<float*>(at + rec + 2 * ml);
+  out->o = reinterpret_cast<float4*>(at + rec + 2 * ml);
   return ATTN_OK;
 }
 

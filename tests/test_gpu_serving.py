@@ -462,6 +462,21 @@ def test_long_request_is_split_and_joined(pkg):
             .check(pkg)
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("Hq,H,new", [(8, 8, 1), (8, 8, 30), (32, 8, 8), (32, 8, 20), (24, 8, 60)])
+def test_blocks_take_several_tiles_and_items(pkg, dtype, cache, Hq, H, new):
+    """More work than blocks: pieces of many tiles, shares that begin and end inside items."""
+    held = [3000, 1, 2048, 2900, 700, 127, 1500]
+    Tree(dtype, cache, Hq, H, 128, 64, held, [new, 1, new, max(1, new // 2), new, 1, new],
+         "tree" if new > 1 else None, seed=new).run(pkg).check(pkg)
+
+
+def test_long_chunks(pkg):
+    """Chains of many row tiles: more items than blocks, accumulators whose keys end at different tiles."""
+    Tree(BF16, BF16, 16, 4, 128, 128, [300, 0], [1300, 900], seed=22).run(pkg).check(pkg)
+    Tree(F16, F16, 8, 8, 64, 64, [600], [2000], seed=23).run(pkg).check(pkg)
+
+
 def test_many_small_requests(pkg):
     Tree(BF16, BF16, 4, 2, 128, 16, [i % 50 for i in range(700)], [i % 3 for i in range(700)], seed=10).run(pkg).check(pkg)
     Tree(F16, F16, 2, 1, 64, 16, [0] * 300, [1] * 300, seed=11).run(pkg).check(pkg)
