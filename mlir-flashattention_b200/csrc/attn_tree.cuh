@@ -32,6 +32,7 @@ struct Params {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;
   int64_t kc_sp, kc_sh, kc_st, vc_sp, vc_sh, vc_st;
   int64_t table_stride, mask_stride;
+  int mask_align;  // bytes that every row of the mask is aligned to
   const void* q;
   const void* k_new;
   const void* v_new;
@@ -117,27 +118,66 @@ __device__ __forceinline__ int64_t head_units(const Params& p, const Split& s, c
 }
 
 // Where a block's share begins, found by the whole block (blockDim.x threads,
-// a multiple of 32, at most 1024).
+// a multiple of 32, at most 1024).  Up to 32 requests every warp finds it for
+// itself, without a barrier: the step of latency that a small call can spare.
 struct Share {
   int64_t lo, hi;  // units still to do
   int64_t off;     // units of request b before lo
   int64_t head;    // units of one of its kv-heads
   int b;           // request that holds unit lo
   Request r;
+  int64_t total;   // units of all blocks with a share, and their number
+  int blocks;
 };
+
+// Units [lo, hi) of block c of `blocks`.
+__device__ __forceinline__ void share_bounds(int64_t total, int blocks, int c, int64_t& lo, int64_t& hi) {
+  if (total < (int64_t{1} << 20) && blocks <= 2048) {  // products below 2^31: no 64-bit division
+    const uint32_t t = static_cast<uint32_t>(total), n = static_cast<uint32_t>(blocks);
+    lo = t * static_cast<uint32_t>(c) / n, hi = t * static_cast<uint32_t>(c + 1) / n;
+  } else {
+    lo = total * c / blocks, hi = total * (c + 1) / blocks;
+  }
+}
+
+__device__ __forceinline__ int64_t scan_warp(int64_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += t;
+  }
+  return v;
+}
 
 __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int min_units) {
   __shared__ int64_t warp_sum[32];
   __shared__ Share found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  auto scan = [&](int64_t v) {
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t t = __shfl_up_sync(0xffffffffu, v, d);
-      if (lane >= d) v += t;
-    }
-    return v;
+  const int c = static_cast<int>(blockIdx.x);
+  auto blocks_for = [&](int64_t total) {
+    return static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + min_units - 1) / min_units));
   };
+  if (p.B <= 32) {
+    Share r{};
+    if (lane < p.B) {
+      r.r = request(p, lane);
+      r.head = head_units(p, s, r.r);
+    }
+    const int64_t units = r.head * p.Hkv, end = scan_warp(units, lane);
+    r.total = __shfl_sync(0xffffffffu, end, 31);
+    r.blocks = blocks_for(r.total);
+    if (c < r.blocks) share_bounds(r.total, r.blocks, c, r.lo, r.hi);
+    r.off = r.lo - (end - units);
+    const unsigned has = __ballot_sync(0xffffffffu, r.off >= 0 && r.lo < end);
+    const int src = has ? __ffs(has) - 1 : 0;
+    r.b = src;
+    r.off = __shfl_sync(0xffffffffu, r.off, src);
+    r.head = __shfl_sync(0xffffffffu, r.head, src);
+    r.r.held = __shfl_sync(0xffffffffu, r.r.held, src);
+    r.r.first = __shfl_sync(0xffffffffu, r.r.first, src);
+    r.r.count = __shfl_sync(0xffffffffu, r.r.count, src);
+    return r;
+  }
   // A thread sums requests tid, tid + threads, ..; with more requests than
   // threads a second pass finds the one that holds the share's first unit.
   const int chunks = (p.B + blockDim.x - 1) / blockDim.x;
@@ -148,7 +188,7 @@ __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int
     head = head_units(p, s, r);
     mine += head * p.Hkv;
   }
-  int64_t inc = scan(mine);
+  int64_t inc = scan_warp(mine, lane);
   if (lane == 31) warp_sum[warp] = inc;
   __syncthreads();
   int64_t total = 0, before = 0;
@@ -156,15 +196,15 @@ __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
-  const int64_t blocks = min(static_cast<int64_t>(gridDim.x), (total + min_units - 1) / min_units);
-  const int64_t c = blockIdx.x;
+  const int blocks = blocks_for(total);
   if (c >= blocks) {
     Share none{};
     return none;
   }
-  const int64_t lo = total * c / blocks, hi = total * (c + 1) / blocks;
+  int64_t lo, hi;
+  share_bounds(total, blocks, c, lo, hi);
   auto offer = [&](int b, int64_t end, int64_t units) {
-    if (end - units <= lo && lo < end) found = Share{lo, hi, lo - (end - units), head, b, r};
+    if (end - units <= lo && lo < end) found = Share{lo, hi, lo - (end - units), head, b, r, total, blocks};
   };
   if (chunks == 1) {
     offer(tid, before + inc, mine);
@@ -177,7 +217,7 @@ __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int
         r = request(p, b);
         head = head_units(p, s, r);
       }
-      inc = scan(head * p.Hkv);
+      inc = scan_warp(head * p.Hkv, lane);
       __syncthreads();
       if (lane == 31) warp_sum[warp] = inc;
       __syncthreads();
@@ -191,6 +231,11 @@ __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int
   }
   __syncthreads();
   return found;
+}
+
+// The block whose share holds unit u.
+__device__ __forceinline__ int block_of(const Share& sh, int64_t u) {
+  return static_cast<int>(((u + 1) * sh.blocks - 1) / sh.total);
 }
 
 // The next piece of a share; moves past it.  False at its end.
@@ -236,18 +281,38 @@ __device__ __forceinline__ bool next_piece(const Params& p, const Split& s, Shar
 }
 
 // Scratch of the pieces that are not whole items: block c's first piece goes
-// to slot 2 c, its last to 2 c + 1.
-struct Record {
-  int b, h, rt;  // b = -1: nothing in this slot
-  int ends;      // bit 0: the item's first piece, bit 1: its last
+// to slot 2 c, its last to 2 c + 1.  The block that holds an item's first
+// piece leaves what the join needs to know.
+struct alignas(32) Record {
+  int pieces;  // 0: no cut item begins in this block
+  int slot;    // of the first piece; the others are the first ones of the blocks that follow
+  int first;   // first row of q of the request
+  int row;     // first query row of the item in the request
+  int rows;
+  int h;
 };
 
 struct Scratch {
-  Record* record;  // [2 blocks]
+  Record* record;  // [blocks]
   float* m;        // [2 blocks][rows] running maximum, log2 units
   float* l;        // [2 blocks][rows]
-  float4* o;       // [2 blocks][D / 4][rows], relative to m, not divided by l
+  float4* o;       // [2 blocks], in the kernel's own order, relative to m, not divided by l
 };
+
+// Called with the share already moved past the piece.
+__device__ __forceinline__ Record make_record(const Params& p, const Split& s, const Share& sh, const Piece& pc,
+                                              int slot) {
+  Record r;
+  const int64_t end = sh.lo + (pc.tiles - pc.k1);  // the item's end
+  r.pieces = block_of(sh, end - 1) - static_cast<int>(blockIdx.x) + 1;
+  r.slot = slot;
+  r.first = pc.r.first;
+  r.row = pc.rt * s.rows;
+  r.rows = static_cast<int>(min(static_cast<int64_t>(s.rows), static_cast<int64_t>(pc.r.count) * p.group -
+                                                                  static_cast<int64_t>(pc.rt) * s.rows));
+  r.h = pc.h;
+  return r;
+}
 
 template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }

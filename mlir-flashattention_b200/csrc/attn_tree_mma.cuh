@@ -101,6 +101,12 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// Programmatic launches: what the kernel before in the stream wrote may be
+// read after grid_wait; the kernel behind may be set up after grid_release (it
+// waits in turn for this one's end).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // The four reading warps meet.
 __device__ __forceinline__ void readers_sync() {
   __syncwarp();
@@ -130,7 +136,6 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
   float* const s_join = reinterpret_cast<float*>(smem + C::kStages * 2 * C::kTile + kMmaRows * D * 2);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       attn_sm100::mbar_init(&full[s], 1);
@@ -140,7 +145,9 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     attn_sm100::fence_mbar_init();
     attn_sm100::fence_proxy_async_smem();
   }
-  if (tid < 2) scratch.record[2 * blockIdx.x + tid].b = -1;
+  grid_wait();
+  grid_release();
+  if (tid == 0) scratch.record[blockIdx.x].pieces = 0;
   Share share = find_share(p, split, min_units);  // synchronises the block
   __syncthreads();
   const int64_t share_lo = share.lo;
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
           uint2 w = make_uint2(pack2<F16>(x.x * inv, x.y * inv), pack2<F16>(x.z * inv, x.w * inv));
           *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + c0 + wc) = w;
         } else {
-          scratch.o[(static_cast<int64_t>(slot) * (D / 4) + (c0 + wc) / 4) * kMmaRows + wr] = x;
+          scratch.o[(static_cast<int64_t>(slot) * kMmaRows + wr) * (D / 4) + (c0 + wc) / 4] = x;
         }
       }
       readers_sync();
@@ -587,91 +594,95 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         scratch.l[slot * kMmaRows + wr] = sum;
       }
     }
-    if (!whole && tid == 0)
-      scratch.record[slot] = Record{pc.b, pc.h, pc.rt, (pc.k0 == 0 ? 1 : 0) | (pc.k1 == pc.tiles ? 2 : 0)};
+    if (!whole && pc.k0 == 0 && tid == 0) scratch.record[blockIdx.x] = make_record(p, split, share, pc, slot);
   }
 }
 
-// Joins the pieces of the items that were cut: block (c, y) takes rows 16 y to
-// 16 y + 15 of the item whose first piece block c of the first kernel ended
-// with, if any; the pieces that follow are the first ones of the blocks after
-// it.  Added in that order, so that a call gives the same bits every time.
-constexpr int kJoinThreads = 256, kJoinRows = 16;
+// Joins the pieces of the items that were cut: block (c, y) takes `rows_each`
+// query rows of the cut item that begins in block c of the first kernel, if
+// any.  What bounds it is latency, a record and then everything else at once:
+// a thread has four columns of a row and every G-th piece of the item, brought
+// to one maximum as it goes; the G parts meet in shared memory.  The order of
+// the sums depends on the lengths alone, so a call gives the same bits every
+// time.
+constexpr int kJoinThreads = 256;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-    tree_join_kernel(const __grid_constant__ Params p, const Scratch scratch, const int split_rows,
-                     const int slot_rows, const float shift) {
+    tree_mma_join(const __grid_constant__ Params p, const Scratch scratch, const int rows_each, const float shift) {
   constexpr bool F16 = std::is_same<T, __half>::value;
-  extern __shared__ float factor[];  // [pieces][16]
-  __shared__ float row_top[kJoinRows], row_sum[kJoinRows];
-  __shared__ int sh_count;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int slot = 2 * c + 1;
-  Record rec = scratch.record[slot];
-  if (rec.b < 0 || rec.ends != 1) {
-    slot = 2 * c;
-    rec = scratch.record[slot];
-    if (rec.b < 0 || rec.ends != 1) return;
-  }
-  const Request r = request(p, rec.b);
-  const int row0 = blockIdx.y * kJoinRows;
-  const int64_t item_rows = min(static_cast<int64_t>(split_rows),
-                                static_cast<int64_t>(r.count) * p.group - static_cast<int64_t>(rec.rt) * split_rows);
-  const int rows = static_cast<int>(min(static_cast<int64_t>(kJoinRows), item_rows - row0));
-  if (rows <= 0) return;
-  if (warp == 0) {
-    int n = 0;
-    for (int at = c + 1;; at += 32) {
-      const bool last = at + lane < static_cast<int>(gridDim.x) && (scratch.record[2 * (at + lane)].ends & 2);
-      const unsigned found = __ballot_sync(0xffffffffu, last);
-      if (found || at + 32 >= static_cast<int>(gridDim.x)) {
-        n = at - c + (found ? __ffs(found) : 0);
-        break;
+  constexpr int kCols = D / 4, kParts = kJoinThreads / kCols;  // threads of a row; rows x G at once
+  __shared__ float4 part_o[kJoinThreads];
+  __shared__ float part_m[kJoinThreads], part_l[kJoinThreads];
+  grid_wait();
+  grid_release();
+  const int c = blockIdx.x, tid = threadIdx.x, col = tid % kCols, part = tid / kCols;
+  const Record rec = scratch.record[c];
+  const int row_lo = blockIdx.y * rows_each, row_hi = min(rec.rows, row_lo + rows_each);
+  if (rec.pieces == 0 || row_lo >= row_hi) return;
+  const int n = rec.pieces;
+  int G = 1;
+  while (G < kParts && 2 * G < n) G *= 2;
+  const int step = kParts / G, g = part % G;
+  for (int base = row_lo; base < row_hi; base += step) {
+    const int row = base + part / G;
+    float top = -INFINITY, sum = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < row_hi) {
+      for (int i0 = g; i0 < n; i0 += 4 * G) {
+        float m[4], l[4];
+        float4 y[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = i0 + x * G;
+          m[x] = -INFINITY, l[x] = 0.f, y[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i < n) {
+            const int s = i == 0 ? rec.slot : 2 * (c + i);
+            m[x] = scratch.m[s * kMmaRows + row];
+            l[x] = scratch.l[s * kMmaRows + row];
+            y[x] = scratch.o[(static_cast<int64_t>(s) * kMmaRows + row) * kCols + col];
+          }
+        }
+        const float high = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
+        if (high != -INFINITY) {
+          const float f = attn_sm100::ex2(top - high);
+          top = high;
+          sum *= f, a.x *= f, a.y *= f, a.z *= f, a.w *= f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float w = attn_sm100::ex2(m[x] - high);
+            sum += w * l[x];
+            a.x += w * y[x].x, a.y += w * y[x].y, a.z += w * y[x].z, a.w += w * y[x].w;
+          }
+        }
       }
     }
-    if (lane == 0) sh_count = n;
-  }
-  __syncthreads();
-  const int n = sh_count;
-  auto slot_of = [&](int i) { return i == 0 ? slot : 2 * (c + i); };
-  for (int x = tid; x < n * rows; x += kJoinThreads) {
-    const int i = x / rows, row = x - i * rows;
-    factor[i * kJoinRows + row] = scratch.m[slot_of(i) * slot_rows + row0 + row];
-  }
-  __syncthreads();
-  for (int row = warp; row < rows; row += kJoinThreads / 32) {
-    float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, factor[i * kJoinRows + row]);
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    for (int i = lane; i < n; i += 32) {
-      const float f = top == -INFINITY ? 0.f : attn_sm100::ex2(factor[i * kJoinRows + row] - top);
-      factor[i * kJoinRows + row] = f;
-      sum += f * scratch.l[slot_of(i) * slot_rows + row0 + row];
+    if (G > 1) {
+      part_o[tid] = a, part_m[tid] = top, part_l[tid] = sum;
+      __syncthreads();
+      if (g == 0) {
+        for (int i = 1; i < G; ++i) {
+          const int o = tid + i * kCols;
+          const float m = part_m[o], high = fmaxf(m, top);
+          if (high == -INFINITY) continue;
+          const float f = attn_sm100::ex2(top - high), w = attn_sm100::ex2(m - high);
+          const float4 y = part_o[o];
+          top = high;
+          sum = sum * f + w * part_l[o];
+          a.x = a.x * f + w * y.x, a.y = a.y * f + w * y.y, a.z = a.z * f + w * y.z, a.w = a.w * f + w * y.w;
+        }
+      }
+      __syncthreads();
     }
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) row_top[row] = top, row_sum[row] = sum;
-  }
-  __syncthreads();
-  for (int x = tid; x < kJoinRows * (D / 4); x += kJoinThreads) {
-    const int row = x & (kJoinRows - 1), col = x / kJoinRows * 4;
-    if (row >= rows) continue;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float f = factor[i * kJoinRows + row];
-      const float4 y = scratch.o[(static_cast<int64_t>(slot_of(i)) * (D / 4) + col / 4) * slot_rows + row0 + row];
-      a.x += f * y.x, a.y += f * y.y, a.z += f * y.z, a.w += f * y.w;
+    if (g == 0 && row < row_hi) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int at = rec.row + row;
+      const int token = rec.first + at / p.group, head = rec.h * p.group + at % p.group;
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + 4 * col) =
+          make_uint2(pack2<F16>(a.x * inv, a.y * inv), pack2<F16>(a.z * inv, a.w * inv));
+      if (col == 0 && p.lse)
+        p.lse[static_cast<int64_t>(token) * p.Hq + head] = sum == 0.f ? -INFINITY : (top - shift + log2f(sum)) * kLn2;
     }
-    const float sum = row_sum[row], inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int at = rec.rt * split_rows + row0 + row;
-    const int token = r.first + at / p.group, head = rec.h * p.group + at % p.group;
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + col) =
-        make_uint2(pack2<F16>(a.x * inv, a.y * inv), pack2<F16>(a.z * inv, a.w * inv));
-    if (col == 0 && p.lse)
-      p.lse[static_cast<int64_t>(token) * p.Hq + head] =
-          sum == 0.f ? -INFINITY : (row_top[row] - shift + log2f(sum)) * kLn2;
   }
 }
 

@@ -77,7 +77,8 @@ struct Job {
   int held, first, count;  // of the request
   int alone;               // one row tile, whose key tiles both accumulators take in turn
   int end0, end1;          // first key tile that accumulator 0 / 1 does not need
-  int rec, ends;           // scratch slot; Record::ends
+  int rec;                 // scratch slot
+  int whole;               // all of its item's key tiles
   int rows;                // query rows of the item
 
   // Accumulator t takes key tile k.
@@ -109,35 +110,57 @@ __device__ __forceinline__ Job make_job(const Params& p, const Split& s, const T
     j.end0 = pc.cached + ((keys + (1 << s.new_shift) - 1) >> s.new_shift);
   }
   j.rec = rec;
-  j.ends = (pc.k0 == 0 ? 1 : 0) | (pc.k1 == pc.tiles ? 2 : 0);
+  j.whole = pc.k0 == 0 && pc.k1 == pc.tiles;
   return j;
 }
 
-// Bits of one row of the mask for keys [first, first + here) of its request's
-// new ones: the warp reads each row of its 32 query rows' tokens together.
-__device__ __forceinline__ void mask_bits(const Params& p, int row0, int token, int t_lo, int t_hi, int first,
-                                          int here, int lane, uint32_t (&bits)[4]) {
+// Bits of one row of the mask for `here` <= 128 new keys (1: masked, or no
+// such key), from V bytes at a time; the row is aligned to V.
+template <int V>
+__device__ __forceinline__ void mask_row(const uint8_t* row, int here, uint32_t (&bits)[4]) {
+  using W = typename std::conditional<V == 16, uint4, typename std::conditional<V == 4, uint32_t, uint8_t>::type>::type;
+  auto nibble = [](uint32_t w) { return ((__vcmpne4(w, 0u) & 0x08040201u) * 0x01010101u) >> 24; };
 #pragma unroll
-  for (int w = 0; w < 4; ++w) bits[w] = 0xffffffffu;
-  const uint8_t* const m = p.mask + static_cast<int64_t>(row0) * p.mask_stride + first;
-  for (int t0 = t_lo; t0 <= t_hi; t0 += 4) {
-    uint32_t b[4][4];
+  for (int q = 0; q < 4; ++q) {
+    uint32_t b = 0;
+    if (32 * q < here) {
+      constexpr int kLoads = 32 / V;
+      W w[kLoads];
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < kLoads; ++x)
+        if (32 * q + (x + 1) * V <= here) w[x] = *reinterpret_cast<const W*>(row + 32 * q + x * V);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        b[x][w] = 1;
-        if (t0 + x <= t_hi && 32 * w + lane < here)
-          b[x][w] = m[static_cast<int64_t>(t0 + x) * p.mask_stride + 32 * w + lane];
+      for (int x = 0; x < kLoads; ++x) {
+        if (32 * q + (x + 1) * V <= here) {
+          if constexpr (V == 16)
+            b |= (nibble(w[x].x) | nibble(w[x].y) << 4 | nibble(w[x].z) << 8 | nibble(w[x].w) << 12) << (16 * x);
+          else if constexpr (V == 4)
+            b |= nibble(w[x]) << (4 * x);
+          else
+            b |= (w[x] != 0 ? 1u : 0u) << x;
+        } else {
+          for (int e = 0; e < V; ++e) {
+            const int j = x * V + e;
+            if (32 * q + j < here && row[32 * q + j] != 0) b |= 1u << j;
+          }
+        }
       }
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t v = __ballot_sync(0xffffffffu, b[x][w] != 0);
-        if (token == t0 + x) bits[w] = v;
-      }
+      if (32 * q + 32 > here) b |= 0xffffffffu << (here - 32 * q);
+    } else {
+      b = 0xffffffffu;
+    }
+    bits[q] = b;
   }
+}
+
+// Not inlined: it runs once or twice an item, and its loads would take the
+// registers of every tile's softmax.
+__device__ __noinline__ uint4 mask_row_bits(const uint8_t* row, int here, int align) {
+  uint32_t b[4];
+  if (align >= 16) mask_row<16>(row, here, b);
+  else if (align >= 4) mask_row<4>(row, here, b);
+  else mask_row<1>(row, here, b);
+  return make_uint4(b[0], b[1], b[2], b[3]);
 }
 
 template <typename T, int D>
@@ -170,7 +193,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   Job* const jobs = reinterpret_cast<Job*>(tmem_slot + 4);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -199,7 +221,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (tid < 2) scratch.record[2 * blockIdx.x + tid].b = -1;
+  grid_wait();
+  grid_release();
+  if (tid == 0) scratch.record[blockIdx.x].pieces = 0;
   tc_fence_before();
   Share share = find_share(p, split, min_units);
   __syncthreads();
@@ -398,7 +422,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = wait(&job_empty[i], static_cast<uint32_t>((n / C::kQueue) & 1) ^ 1u);
         if (!ok) break;
         if (lane == 0) {
-          if (more) jobs[i] = make_job(p, split, tiles, pc, 2 * blockIdx.x + (lo == share_lo ? 0 : 1));
+          const int rec = 2 * blockIdx.x + (lo == share_lo ? 0 : 1);
+          if (more && pc.k0 == 0 && pc.k1 < pc.tiles)
+            scratch.record[blockIdx.x] = make_record(p, split, share, pc, rec);
+          if (more) jobs[i] = make_job(p, split, tiles, pc, rec);
           else jobs[i].b = -1;
           mbar_arrive(&job_full[i]);
         }
@@ -436,9 +463,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int here = j.here(split, k);
         uint32_t bits[4];
         const bool masked = !cached && p.mask != nullptr && busy;
-        if (masked)
-          mask_bits(p, j.first, token, __shfl_sync(0xffffffffu, token, 0), __shfl_sync(0xffffffffu, token, 31),
-                    (k - j.cached) << split.new_shift, here, lane, bits);
+        if (masked) {
+          const uint8_t* const row = p.mask + static_cast<int64_t>(j.first + token) * p.mask_stride +
+                                     ((k - j.cached) << split.new_shift);
+          const uint4 b = mask_row_bits(row, here, p.mask_align);
+          bits[0] = b.x, bits[1] = b.y, bits[2] = b.z, bits[3] = b.w;
+        }
         ok = wait(&s_full[t], static_cast<uint32_t>(steps & 1));
         if (!ok) break;
         tc_fence_after();
@@ -556,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       base += 2 * (j.k1 - j.k0);
       // ------------------------------------------------------------ a piece ends
-      const bool has = from < stop, whole = j.ends == 3;
+      const bool has = from < stop, whole = j.whole;
       if (has && !wait(&pv_done[t], static_cast<uint32_t>((steps - 1) & 1))) break;
       tc_fence_after();
       // Alone: columns [D/2 t, D/2 t + D/2) of both accumulators; else all of its own.
@@ -631,12 +661,78 @@ __global__ void __launch_bounds__(kThreads, 1)
               none ? -INFINITY : (mm - C::kShift + log2f(ll)) * kLn2;
         }
       }
-      if (!whole && tid == 0) scratch.record[j.rec] = Record{j.b, j.h, j.rt, j.ends};
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// The join of this kernel's cut items: block (c, y) takes 32 query rows of the
+// cut item that begins in block c of the first kernel, if any.  A lane is a
+// row (as the first kernel stores them), a warp has D / 4 / 16 times four
+// columns; an item has few pieces (all of them only where a single item fills
+// the GPU), so a thread reads four of each column at once and adds in order.
+constexpr int kJoinThreads = 512, kJoinRows = 32;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+    tree_tc_join(const __grid_constant__ Params p, const Scratch scratch) {
+  using C = Cfg<T, D>;
+  constexpr int kCols = D / 4 / (kJoinThreads / 32);
+  grid_wait();
+  grid_release();
+  const int c = blockIdx.x, lane = threadIdx.x & 31, col = (threadIdx.x >> 5) * kCols;
+  const Record rec = scratch.record[c];
+  const int row = blockIdx.y * kJoinRows + lane;
+  if (rec.pieces == 0 || row >= rec.rows) return;
+  const int n = rec.pieces;
+  float top = -INFINITY, sum = 0.f;
+  float4 a[kCols] = {};
+  for (int i0 = 0; i0 < n; i0 += 4) {
+    float m[4], l[4];
+    float4 y[4][kCols];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      m[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) y[x][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + x < n) {
+        const int64_t s = i0 + x == 0 ? rec.slot : 2 * (c + i0 + x);
+        m[x] = scratch.m[s * 256 + row];
+        l[x] = scratch.l[s * 256 + row];
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) y[x][k] = scratch.o[(s * (D / 4) + col + k) * 256 + row];
+      }
+    }
+    const float high = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
+    if (high != -INFINITY) {
+      const float f = ex2(top - high);
+      top = high;
+      sum *= f;
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) a[k].x *= f, a[k].y *= f, a[k].z *= f, a[k].w *= f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float w = ex2(m[x] - high);
+        sum += w * l[x];
+#pragma unroll
+        for (int k = 0; k < kCols; ++k)
+          a[k].x += w * y[x][k].x, a[k].y += w * y[x][k].y, a[k].z += w * y[x][k].z, a[k].w += w * y[x][k].w;
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int at = rec.row + row;
+  const int token = rec.first + at / p.group, head = rec.h * p.group + at % p.group;
+  T* const out = static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + 4 * col;
+#pragma unroll
+  for (int k = 0; k < kCols; ++k)
+    reinterpret_cast<uint2*>(out)[k] =
+        make_uint2(pack2<C::F16>(a[k].x * inv, a[k].y * inv), pack2<C::F16>(a[k].z * inv, a[k].w * inv));
+  if (col == 0 && p.lse)
+    p.lse[static_cast<int64_t>(token) * p.Hq + head] =
+        sum == 0.f ? -INFINITY : (top - C::kShift + log2f(sum)) * kLn2;
 }
 
 }  // namespace tc

@@ -5,6 +5,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
+#include <utility>
 
 #include "attn_tree_mma.cuh"
 #include "attn_tree_tc.cuh"
@@ -420,7 +421,7 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Scratch for the cut items of a launch of `blocks` blocks.
 int tree_scratch(attn_tree::Scratch* out, void** base, int blocks, int rows, int D, cudaStream_t s) {
   const size_t slots = 2 * static_cast<size_t>(blocks);
-  const size_t rec = round256(slots * sizeof(attn_tree::Record)), ml = round256(slots * rows * sizeof(float));
+  const size_t rec = round256(blocks * sizeof(attn_tree::Record)), ml = round256(slots * rows * sizeof(float));
   const cudaError_t e = rt_host::scratch(base, rec + 2 * ml + slots * rows * D * sizeof(float), s);
   if (e != cudaSuccess) return cuda_fail(e, "stream-ordered scratch (cut items)");
   char* at = static_cast<char*>(*base);
@@ -431,21 +432,33 @@ int tree_scratch(attn_tree::Scratch* out, void** base, int blocks, int rows, int
   return ATTN_OK;
 }
 
-// The join, launched so that it is set up while the first kernel still runs.
-template <typename T, int D>
-cudaError_t launch_join(const attn_tree::Params& p, const attn_tree::Scratch& sc, int split_rows, int slot_rows,
-                        float shift, int blocks, cudaStream_t s) {
+// Programmatic launch: the kernel is set up while the one before it in the
+// stream still runs, and waits on the device for that one's end.
+template <typename... K, typename... A>
+cudaError_t launch_early(void (*kern)(K...), dim3 grid, int threads, size_t smem, cudaStream_t s, A&&... args) {
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks, (split_rows + attn_tree::kJoinRows - 1) / attn_tree::kJoinRows);
-  cfg.blockDim = dim3(attn_tree::kJoinThreads);
-  cfg.dynamicSmemBytes = sizeof(float) * blocks * attn_tree::kJoinRows;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_tree::tree_join_kernel<T, D>, p, sc, split_rows, slot_rows, shift);
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+
+// Both kernels keep the SM's memory split as the first one needs it: a change
+// of it between them would drain the SM.
+template <typename K, typename J>
+cudaError_t prepare_kernels(K kern, J join, size_t smem) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(join, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  return e;
 }
 
 int pow2_shift(int64_t n, int lo, int hi) {
@@ -462,8 +475,7 @@ int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, const rt_host
   static std::once_flag once[64];
   static cudaError_t attr[64];
   std::call_once(once[dev.index], [&] {
-    attr[dev.index] =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
+    attr[dev.index] = prepare_kernels(kern, attn_tree::tree_mma_join<T, D>, C::kSmem);
   });
   if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "cudaFuncSetAttribute");
   attn_tree::Split split;
@@ -474,12 +486,20 @@ int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, const rt_host
   int rc = make_key_maps(&m, d, std::min(1 << p.page_shift, attn_tree::kMmaKeys), 1 << split.new_shift, true);
   if (rc != ATTN_OK) return rc;
   const int blocks = 2 * dev.sms;
+  const int rows = static_cast<int>(std::min<int64_t>(kRows, static_cast<int64_t>(p.max_new) * p.group));
   attn_tree::Scratch sc{};
   void* base = nullptr;
   if ((rc = tree_scratch(&sc, &base, blocks, kRows, D, s)) != ATTN_OK) return rc;
-  kern<<<blocks, attn_tree::kMmaThreads, C::kSmem, s>>>(m.kc, m.vc, m.kn, m.vn, p, split, sc, 1);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) e = launch_join<T, D>(p, sc, kRows, kRows, C::kShift, blocks, s);
+  cudaError_t e = launch_early(kern, dim3(blocks), attn_tree::kMmaThreads, C::kSmem, s, m.kc, m.vc, m.kn, m.vn, p,
+                               split, sc, 1);
+  if (e == cudaSuccess) {
+    // Rows of a join block: about twice the blocks that fit at once; more
+    // would come too late to hide their start.
+    const int at_once = dev.sms * (2048 / attn_tree::kJoinThreads);
+    const int each = std::max(1, blocks * rows / (2 * at_once));
+    e = launch_early(attn_tree::tree_mma_join<T, D>, dim3(blocks, (rows + each - 1) / each), attn_tree::kJoinThreads, 0,
+                     s, p, sc, each, C::kShift);
+  }
   cudaFreeAsync(base, s);
   if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
   rt_host::count_launches(2);
@@ -495,8 +515,7 @@ int launch_tree_tc(const AttnTree& d, const attn_tree::Params& p, const rt_host:
   static int regs[64];
   std::call_once(once[dev.index], [&] {
     cudaFuncAttributes fa{};
-    attr[dev.index] =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem));
+    attr[dev.index] = prepare_kernels(kern, attn_tree::tc::tree_tc_join<T, D>, C::kSmem);
     if (attr[dev.index] == cudaSuccess) attr[dev.index] = cudaFuncGetAttributes(&fa, kern);
     regs[dev.index] = fa.numRegs;
   });
@@ -523,12 +542,16 @@ int launch_tree_tc(const AttnTree& d, const attn_tree::Params& p, const rt_host:
   const CUtensorMapDataType t16 = C::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   if ((rc = make_map(&mq, d.q, t16, dims, strides, box)) != ATTN_OK) return rc;
   const int blocks = dev.sms;
+  const int rows = static_cast<int>(std::min<int64_t>(split.rows, static_cast<int64_t>(p.max_new) * p.group));
   attn_tree::Scratch sc{};
   void* base = nullptr;
   if ((rc = tree_scratch(&sc, &base, blocks, 256, D, s)) != ATTN_OK) return rc;
-  kern<<<blocks, attn_tree::tc::kThreads, C::kSmem, s>>>(mq, m.kc, m.vc, m.kn, m.vn, p, split, tiles, sc, 1);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) e = launch_join<T, D>(p, sc, split.rows, 256, C::kShift, blocks, s);
+  cudaError_t e = launch_early(kern, dim3(blocks), attn_tree::tc::kThreads, C::kSmem, s, mq, m.kc, m.vc, m.kn, m.vn,
+                               p, split, tiles, sc, 1);
+  if (e == cudaSuccess)
+    e = launch_early(attn_tree::tc::tree_tc_join<T, D>,
+                     dim3(blocks, (rows + attn_tree::tc::kJoinRows - 1) / attn_tree::tc::kJoinRows),
+                     attn_tree::tc::kJoinThreads, 0, s, p, sc);
   cudaFreeAsync(base, s);
   if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
   rt_host::count_launches(2);
@@ -562,6 +585,9 @@ int run(const AttnTree& d, cudaStream_t s) {
   p.vc_sp = d.v_cache_stride[0], p.vc_sh = d.v_cache_stride[1], p.vc_st = d.v_cache_stride[2];
   p.table_stride = d.table_stride;
   p.mask_stride = d.mask_stride;
+  p.mask_align = d.T > 1 ? static_cast<int>((reinterpret_cast<uintptr_t>(d.mask) | d.mask_stride) & 15u)
+                         : static_cast<int>(reinterpret_cast<uintptr_t>(d.mask) & 15u);
+  p.mask_align = p.mask_align == 0 ? 16 : p.mask_align & -p.mask_align;
   p.q = d.q, p.k_new = d.k_new, p.v_new = d.v_new;
   p.k_cache = d.k_cache, p.v_cache = d.v_cache;
   p.o = d.o, p.lse = d.lse;

@@ -127,6 +127,7 @@ def test_plan_in_a_graph_decodes_step_by_step(pkg):
                        slots=out[0], positions=out[1], starts=out[2])
         targets.add_(1)
 
+    check_plan(pkg, [5], [2], [[4]], [-1], 0, 16, 0)  # a device's first call is made outside capture
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         step()
