@@ -75,10 +75,11 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
 // request is its token r / group with the kv-head's q-head r % group, so that
 // the heads that share keys share the tile.  Its units are tiles of keys: the
 // cached ones in order, then the new ones it can see.  The units of all items,
-// one after another, are cut into one equal share per block whatever the
-// requests' lengths; a share may begin and end inside an item.  A block meets
-// its share as pieces; one that is not a whole item goes to scratch, and the
-// join (a second kernel) adds up the pieces of each cut item in order.
+// one after another, are cut into equal shares, one for each block (or half of
+// a block), whatever the requests' lengths; a share may begin and end inside an
+// item.  A block meets its share as pieces; one that is not a whole item goes
+// to scratch, and the join (a second kernel) adds up the pieces of each cut
+// item in order.
 struct Split {
   int rows;        // query rows of a tile
   int keys_shift;  // cached keys of a tile, log2
@@ -149,15 +150,18 @@ __device__ __forceinline__ int64_t scan_warp(int64_t v, int lane) {
   return v;
 }
 
-__device__ __forceinline__ Share find_share(const Params& p, const Split& s, int min_units) {
+// TEAMS: shares of a block; a thread gets the share of `team`.  Shares are
+// numbered TEAMS * block + team.
+template <int TEAMS>
+__device__ __forceinline__ Share find_share(const Params& p, const Split& s, int min_units, int team) {
   __shared__ int64_t warp_sum[32];
-  __shared__ Share found;
+  __shared__ Share found[TEAMS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  const int c = static_cast<int>(blockIdx.x);
   auto blocks_for = [&](int64_t total) {
-    return static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + min_units - 1) / min_units));
+    return static_cast<int>(min(static_cast<int64_t>(gridDim.x) * TEAMS, (total + min_units - 1) / min_units));
   };
   if (p.B <= 32) {
+    const int c = static_cast<int>(blockIdx.x) * TEAMS + team;
     Share r{};
     if (lane < p.B) {
       r.r = request(p, lane);
@@ -197,14 +201,19 @@ __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int
     total += warp_sum[w];
   }
   const int blocks = blocks_for(total);
-  if (c >= blocks) {
-    Share none{};
-    return none;
+  int64_t lo[TEAMS], hi[TEAMS];
+#pragma unroll
+  for (int t = 0; t < TEAMS; ++t) {
+    const int c = static_cast<int>(blockIdx.x) * TEAMS + t;
+    lo[t] = hi[t] = -1;
+    if (c < blocks) share_bounds(total, blocks, c, lo[t], hi[t]);
+    else if (tid == 0) found[t] = Share{};
   }
-  int64_t lo, hi;
-  share_bounds(total, blocks, c, lo, hi);
   auto offer = [&](int b, int64_t end, int64_t units) {
-    if (end - units <= lo && lo < end) found = Share{lo, hi, lo - (end - units), head, b, r, total, blocks};
+#pragma unroll
+    for (int t = 0; t < TEAMS; ++t)
+      if (lo[t] >= 0 && end - units <= lo[t] && lo[t] < end)
+        found[t] = Share{lo[t], hi[t], lo[t] - (end - units), head, b, r, total, blocks};
   };
   if (chunks == 1) {
     offer(tid, before + inc, mine);
@@ -230,11 +239,11 @@ __device__ __forceinline__ Share find_share(const Params& p, const Split& s, int
     }
   }
   __syncthreads();
-  return found;
+  return found[team];
 }
 
-// The block whose share holds unit u.
-__device__ __forceinline__ int block_of(const Share& sh, int64_t u) {
+// The number of the share that holds unit u.
+__device__ __forceinline__ int share_of(const Share& sh, int64_t u) {
   return static_cast<int>(((u + 1) * sh.blocks - 1) / sh.total);
 }
 
@@ -280,12 +289,12 @@ __device__ __forceinline__ bool next_piece(const Params& p, const Split& s, Shar
   return true;
 }
 
-// Scratch of the pieces that are not whole items: block c's first piece goes
-// to slot 2 c, its last to 2 c + 1.  The block that holds an item's first
+// Scratch of the pieces that are not whole items: share c's first piece goes
+// to slot 2 c, its last to 2 c + 1.  The share that holds an item's first
 // piece leaves what the join needs to know.
 struct alignas(32) Record {
-  int pieces;  // 0: no cut item begins in this block
-  int slot;    // of the first piece; the others are the first ones of the blocks that follow
+  int pieces;  // 0: no cut item begins in this share
+  int slot;    // of the first piece; the others are the first ones of the shares that follow
   int first;   // first row of q of the request
   int row;     // first query row of the item in the request
   int rows;
@@ -293,18 +302,18 @@ struct alignas(32) Record {
 };
 
 struct Scratch {
-  Record* record;  // [blocks]
-  float* m;        // [2 blocks][rows] running maximum, log2 units
-  float* l;        // [2 blocks][rows]
-  float4* o;       // [2 blocks], in the kernel's own order, relative to m, not divided by l
+  Record* record;  // [shares]
+  float* m;        // [2 shares][rows] running maximum, log2 units
+  float* l;        // [2 shares][rows]
+  float4* o;       // [2 shares], in the kernel's own order, relative to m, not divided by l
 };
 
-// Called with the share already moved past the piece.
-__device__ __forceinline__ Record make_record(const Params& p, const Split& s, const Share& sh, const Piece& pc,
+// Of share c, which has already moved past the piece.
+__device__ __forceinline__ Record make_record(const Params& p, const Split& s, const Share& sh, const Piece& pc, int c,
                                               int slot) {
   Record r;
   const int64_t end = sh.lo + (pc.tiles - pc.k1);  // the item's end
-  r.pieces = block_of(sh, end - 1) - static_cast<int>(blockIdx.x) + 1;
+  r.pieces = share_of(sh, end - 1) - c + 1;
   r.slot = slot;
   r.first = pc.r.first;
   r.row = pc.rt * s.rows;

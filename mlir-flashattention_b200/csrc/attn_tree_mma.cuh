@@ -4,23 +4,29 @@
 // With 16 query rows a cached key of D values costs 4 * 16 * D operations for
 // 4 * D bytes: 16 a byte against the 250 a byte that this GPU can do per byte
 // it reads, so the kernel is bound by the cache's bytes and everything here
-// serves to keep loads in flight: a block is one warp that issues TMA loads of
-// page segments into a ring of tiles (64 keys of K and of V each, 128-byte
-// swizzle) and four warps that each take 16 of a tile's keys, with their own
-// running maximum, sum and accumulators, and meet only when a piece ends.  Two
-// blocks share an SM.  Tensor cores by mma.sync m16n8k16: operands go from
+// serves to keep loads in flight: a team is one warp that issues TMA loads of
+// page segments into a ring of tiles (16 KB of K and of V each, 128-byte
+// swizzle) and four warps that each take a quarter of a tile's keys, with their
+// own running maxima, sums and accumulators, and meet only when a piece ends.
+// A block is two teams and fills an SM; its registers are divided so that the
+// reading warps have 224 (setmaxnreg).  Tensor cores by mma.sync m16n8k16: operands go from
 // shared memory to registers, so 16 rows cost 16 rows (a 128-row accumulator
-// in tensor memory would be 1/8 used and its softmax one warp's work).
+// in tensor memory would be 1/8 used and its softmax one warp's work).  MT
+// 16-row tiles share every key that is read: 1 (decode), 2, or 4 at D = 64,
+// where mma.sync's own rate (a quarter of tcgen05's) still keeps up with the
+// memory; beyond, attn_tree_tc.cuh.
 //
 // An e4m3 cache is met in f16: e4m3 values are f16 values, and a bf16 row of q
 // scaled by the power of two that brings its largest value to 2^14..2^15 is
 // exact in f16 down to 2^-39 of that value.  New keys and values are 16-bit
-// and met in their own type.
+// and met in their own type.  A tile is twice as many keys, so a warp has two
+// groups of 16 at once (MT = 1): the conversions' latency, not their number,
+// was the bound.
 //
 // Weights are rounded to the operands' type for P V.  In bf16 a rounding by
 // 2^-9 would double the error of the result, whose own rounding is the same
-// size: P goes in as two bf16 parts, p and p - bf16(p), for twice the small
-// product's work.
+// size: for one row tile P goes in as two bf16 parts, p and p - bf16(p), for
+// twice the small product's work.
 #pragma once
 
 #include <type_traits>
@@ -30,22 +36,34 @@
 
 namespace attn_tree {
 
-constexpr int kMmaRows = 16, kMmaKeys = 64, kMmaWarps = 4;
-constexpr int kMmaThreads = 32 * (kMmaWarps + 1);
+constexpr int kMmaWarps = 4, kMmaTeams = 2;
+constexpr int kMmaThreads = 384;  // two teams of readers; warps 8 and 9 load, 10 and 11 idle
+constexpr int kMmaRegsRead = 224, kMmaRegsLoad = 56;
+constexpr int kMmaRegPool = 256 * kMmaRegsRead + 128 * kMmaRegsLoad;
 
-template <typename T, typename TC, int D>
+template <typename T, typename TC, int D, int MT>
 struct MmaCfg {
+  static constexpr bool F16 = std::is_same<T, __half>::value;
   static constexpr bool FP8 = sizeof(TC) == 1;
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kKeysShift = FP8 ? 7 : 6;       // cached keys of a tile, log2
+  static constexpr int kGroups = (1 << kKeysShift) / (16 * kMmaWarps);  // of 16 keys, a warp
+  static constexpr int kAtOnce = MT == 1 ? kGroups : 1;
   static constexpr int kRowBytes = D * static_cast<int>(sizeof(TC));
   static constexpr int kNewRowBytes = D * 2;
-  // One operand's part of a stage: 64 cached keys, or as many new ones as fit.
-  static constexpr int kTile = kMmaKeys * kRowBytes;
+  static constexpr int kTile = kRowBytes << kKeysShift;  // K or V of a stage
   static constexpr int kStages = 98304 / (2 * kTile);
-  static constexpr int kNewKeys = kTile / kNewRowBytes;  // most new keys of a stage
-  static constexpr int kJoin = kMmaWarps * kMmaRows * 32 * 4;  // 32 columns of each warp
+  static constexpr int kNewShift = 6;                  // most new keys of a tile, log2
+  static constexpr int kJoinCols = MT == 1 ? 32 : 16;  // columns that the warps join at a time
+  static constexpr int kJoin = kMmaWarps * 16 * kJoinCols * 4;
   // Weights are kept times 2^kShift: in f16 they stay normal down to 2^-22.
-  static constexpr float kShift = (FP8 || std::is_same<T, __half>::value) ? 8.f : 0.f;
-  static constexpr size_t kSmem = 1024 + kStages * 2 * kTile + kMmaRows * D * 2 + kJoin;
+  static constexpr float kShift = (FP8 || F16) ? 8.f : 0.f;
+  static constexpr bool kTwoParts = !F16 && !FP8 && MT == 1;  // P as two bf16 parts
+  static constexpr int kTeam = kStages * 2 * kTile + kRows * D * 2 + kJoin;
+  static constexpr size_t kSmem = 1024 + kMmaTeams * kTeam;
+  static_assert(kTeam % 1024 == 0, "the rings start on swizzle periods");
+  static_assert(kSmem + 4096 <= 232448, "shared memory budget");
+  static_assert((kNewRowBytes << kNewShift) <= kTile, "new keys of a stage");
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -66,12 +84,12 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 template <bool F16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                  "{%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                  "{%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -107,53 +125,65 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// The four reading warps meet.
-__device__ __forceinline__ void readers_sync() {
+// The four reading warps of a team meet.
+__device__ __forceinline__ void readers_sync(int team) {
   __syncwarp();
-  asm volatile("barrier.sync 1, 128;" ::: "memory");
+  asm volatile("barrier.sync %0, 128;" ::"r"(team + 1) : "memory");
 }
 
-template <typename T, typename TC, int D>
-__global__ void __launch_bounds__(kMmaThreads, 2)
+template <typename T, typename TC, int D, int MT>
+__global__ void __launch_bounds__(kMmaThreads, 1)
     tree_mma_kernel(const __grid_constant__ CUtensorMap map_kc, const __grid_constant__ CUtensorMap map_vc,
                     const __grid_constant__ CUtensorMap map_kn, const __grid_constant__ CUtensorMap map_vn,
                     const __grid_constant__ Params p, const Split split, const Scratch scratch,
                     const int min_units) {
-  using C = MmaCfg<T, TC, D>;
-  constexpr bool F16 = std::is_same<T, __half>::value;
-  constexpr bool FP8 = C::FP8;
-  constexpr int kSteps = D / 16;              // k-steps of Q K
-  constexpr int kTilesD = D / 8;              // n-tiles of P V
+  using C = MmaCfg<T, TC, D, MT>;
+  constexpr bool F16 = C::F16, FP8 = C::FP8;
+  constexpr int NG = C::kAtOnce;
+  constexpr int kSteps = D / 16;    // k-steps of Q K
+  constexpr int kTilesD = D / 8;    // n-tiles of P V
+  constexpr bool kHoldQ = MT == 1;  // q's fragments stay in registers
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[C::kStages], empty[C::kStages];
+  __shared__ uint64_t sh_full[kMmaTeams][C::kStages], sh_empty[kMmaTeams][C::kStages];
   __shared__ volatile int abort_flag;
-  __shared__ float warp_m[kMmaWarps][kMmaRows], warp_l[kMmaWarps][kMmaRows];
-  __shared__ float q_unit[kMmaRows];  // e4m3: the power of two that a row of q was divided by
+  __shared__ float sh_m[kMmaTeams][kMmaWarps][C::kRows], sh_l[kMmaTeams][kMmaWarps][C::kRows];
+  __shared__ float sh_unit[kMmaTeams][C::kRows];
 
-  uint8_t* smem = raw + ((1024u - (attn_sm100::smem_u32(raw) & 1023u)) & 1023u);
+  const int lane = threadIdx.x & 31, block_warp = threadIdx.x >> 5;
+  const int team = block_warp < 8 ? block_warp >> 2 : block_warp & 1;
+  const int tid = threadIdx.x & 127, warp = tid >> 5;  // of a reader in its team
+  const int sid = kMmaTeams * blockIdx.x + team;       // this team's share
+  uint64_t* const full = sh_full[team];
+  uint64_t* const empty = sh_empty[team];
+  float (*const warp_m)[C::kRows] = sh_m[team];
+  float (*const warp_l)[C::kRows] = sh_l[team];
+  float* const q_unit = sh_unit[team];  // e4m3: the power of two that a row of q was divided by
+  uint8_t* smem = raw + ((1024u - (attn_sm100::smem_u32(raw) & 1023u)) & 1023u) + team * C::kTeam;
   const uint32_t s_ring = attn_sm100::smem_u32(smem);
-  T* const s_q = reinterpret_cast<T*>(smem + C::kStages * 2 * C::kTile);  // [16][D], chunks swizzled
-  float* const s_join = reinterpret_cast<float*>(smem + C::kStages * 2 * C::kTile + kMmaRows * D * 2);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint8_t* const s_q = smem + C::kStages * 2 * C::kTile;  // [rows][D] of T, chunks swizzled
+  float* const s_join = reinterpret_cast<float*>(s_q + C::kRows * D * 2);
 
-  if (tid == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      attn_sm100::mbar_init(&full[s], 1);
-      attn_sm100::mbar_init(&empty[s], kMmaWarps);
-    }
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < kMmaTeams; ++t)
+      for (int s = 0; s < C::kStages; ++s) {
+        attn_sm100::mbar_init(&sh_full[t][s], 1);
+        attn_sm100::mbar_init(&sh_empty[t][s], kMmaWarps);
+      }
     abort_flag = 0;
     attn_sm100::fence_mbar_init();
     attn_sm100::fence_proxy_async_smem();
   }
   grid_wait();
   grid_release();
-  if (tid == 0) scratch.record[blockIdx.x].pieces = 0;
-  Share share = find_share(p, split, min_units);  // synchronises the block
+  if (threadIdx.x < kMmaTeams) scratch.record[kMmaTeams * blockIdx.x + threadIdx.x].pieces = 0;
+  Share share = find_share<kMmaTeams>(p, split, min_units, team);
   __syncthreads();
   const int64_t share_lo = share.lo;
   Piece pc;
 
-  if (warp == kMmaWarps) {
+  if (block_warp >= 8) {
+    attn_sm100::setmaxnreg_dec<kMmaRegsLoad>();
+    if (block_warp >= 10) return;
     // ------------------------------------------------------------- producer
     if (lane == 0) {
       attn_sm100::prefetch_tmap(&map_kc);
@@ -163,27 +193,31 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     }
     const int seg_shift = min(p.page_shift, split.keys_shift);  // rows of a page segment, log2
     const int seg_bytes = C::kRowBytes << seg_shift;
-    int64_t n = 0;  // stages filled
+    int n = 0;  // stages filled
     bool ok = true;
     while (ok && next_piece(p, split, share, pc)) {
       const int32_t* const row = p.table + pc.b * p.table_stride;
+      auto segments = [&](int k) {
+        return (min(1 << split.keys_shift, pc.r.held - (k << split.keys_shift)) + (1 << seg_shift) - 1) >> seg_shift;
+      };
+      auto page_of = [&](int k) {  // of this lane's segment
+        if (k >= min(pc.cached, pc.k1) || lane >= segments(k)) return 0;
+        return __ldg(row + (((k << split.keys_shift) + (lane << seg_shift)) >> p.page_shift));
+      };
+      int page_next = page_of(pc.k0);
       for (int k = pc.k0; k < pc.k1 && ok; ++k, ++n) {
-        const int s = static_cast<int>(n % C::kStages);
+        const int s = n % C::kStages;
         const uint32_t u = static_cast<uint32_t>(n / C::kStages);
         const bool cached = k < pc.cached;
         const int first = cached ? k << split.keys_shift : (k - pc.cached) << split.new_shift;
-        // Page ids before the wait: the loads overlap it.
-        int segs = 1, page = 0, at = 0;
-        if (cached) {
-          segs = (min(1 << split.keys_shift, pc.r.held - first) + (1 << seg_shift) - 1) >> seg_shift;
-          if (lane < segs) {
-            const int key = first + (lane << seg_shift);
-            page = __ldg(row + (key >> p.page_shift));
-            at = key & ((1 << p.page_shift) - 1);
-            if (page < 0 || page >= p.num_pages) {
-              atomicCAS(p.status, 0, ATTN_ERR_INVALID);
-              page = max(p.num_pages, 1);  // outside the map: zeros
-            }
+        const int segs = cached ? segments(k) : 1;
+        int page = page_next, at = 0;
+        page_next = page_of(k + 1);  // a tile ahead of its use
+        if (cached && lane < segs) {
+          at = (first + (lane << seg_shift)) & ((1 << p.page_shift) - 1);
+          if (page < 0 || page >= p.num_pages) {
+            atomicCAS(p.status, 0, ATTN_ERR_INVALID);
+            page = max(p.num_pages, 1);  // outside the map: zeros
           }
         }
         ok = __all_sync(0xffffffffu, attn_sm100::mbar_wait_bounded(&empty[s], (u & 1u) ^ 1u, &abort_flag,
@@ -215,31 +249,30 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     return;
   }
 
+  attn_sm100::setmaxnreg_inc<kMmaRegsRead>();
   // ------------------------------------------------------------- four readers
   const int quad = lane & 3, grp = lane >> 2;
-  int64_t n = 0;
+  const uint32_t s_q32 = attn_sm100::smem_u32(s_q);
+  const float scale2 = p.scale * kLog2e;
+  int n = 0;
   bool ok = true;
   while (next_piece(p, split, share, pc)) {
+    const int row0 = pc.rt * C::kRows;  // the item's first row in the request
     const int rows = static_cast<int>(
-        min(static_cast<int64_t>(kMmaRows), static_cast<int64_t>(pc.r.count) * p.group - pc.rt * kMmaRows));
-    auto row_of = [&](int r, int& token, int& head) {
-      const int at = pc.rt * kMmaRows + r;
-      token = pc.r.first + at / p.group;
-      head = pc.h * p.group + at % p.group;
-    };
+        min(static_cast<int64_t>(C::kRows), static_cast<int64_t>(pc.r.count) * p.group - row0));
     // q rows to shared memory (rows behind the last: zeros), 8 threads a row.
-    {
-      const int r = tid >> 3;
-      int token, head;
-      row_of(r, token, head);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = 16 * mt + (tid >> 3), at = row0 + r;
+      const T* const src = static_cast<const T*>(p.q) + static_cast<int64_t>(pc.r.first + at / p.group) * p.q_st +
+                           (pc.h * p.group + at % p.group) * p.q_sh;
       uint4 v[D / 64];
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         const int chunk = (tid & 7) + 8 * c;
         v[c] = make_uint4(0, 0, 0, 0);
-        if (r < rows)
-          v[c] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + token * p.q_st + head * p.q_sh) + chunk);
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(s_q) + r * D * 2 + ((chunk ^ (r & 7)) * 16)) = v[c];
+        if (r < rows) v[c] = __ldg(reinterpret_cast<const uint4*>(src) + chunk);
+        *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((chunk ^ (r & 7)) * 16)) = v[c];
       }
       if constexpr (FP8 && !F16) {
         float top = 0.f;
@@ -258,250 +291,328 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
         if ((tid & 7) == 0) q_unit[r] = __uint_as_float(static_cast<uint32_t>(e) << 23);
       }
     }
-    readers_sync();
-    // A fragments of q.  For an e4m3 cache the order of d is the one in which
-    // a thread finds 16 of a key's values in one load (see below).
-    uint32_t qa[kSteps][4];
-    const uint32_t s_q32 = attn_sm100::smem_u32(s_q);
-    auto q_frag = [&](uint32_t (&a)[4], int s) {  // 16-bit keys: plain order
-      const int r = (lane & 7) + 8 * ((lane >> 3) & 1), chunk = 2 * s + (lane >> 4);
+    readers_sync(team);
+    // A fragments of 16 rows of q and one k-step, in q's own type and order.
+    auto q_frag = [&](uint32_t (&a)[4], int mt, int s) {
+      const int r = 16 * mt + (lane & 7) + 8 * ((lane >> 3) & 1), chunk = 2 * s + (lane >> 4);
       ldmatrix4(a, s_q32 + r * D * 2 + ((chunk ^ (r & 7)) * 16));
     };
-    float unit[2] = {1.f, 1.f};
-    if constexpr (FP8) {
-      float inv[2] = {1.f, 1.f};
-      if constexpr (!F16) {
-        unit[0] = q_unit[grp], unit[1] = q_unit[grp + 8];
-        inv[0] = 1.f / unit[0], inv[1] = 1.f / unit[1];
-      }
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int d = (s >> 2) * 64 + quad * 16 + (s & 3) * 4;  // 4 values from here
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = grp + 8 * x;
-          const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(s_q) + r * D * 2 +
-                                                          (((d >> 3) ^ (r & 7)) * 16) + (d & 7) * 2);
-          if constexpr (F16) {
-            qa[s][x] = w.x, qa[s][2 + x] = w.y;
-          } else {
-            auto half2 = [&](uint32_t b) {
-              return attn_sm100::pack_f16(__uint_as_float(b << 16) * inv[x], __uint_as_float(b & 0xffff0000u) * inv[x]);
-            };
-            qa[s][x] = half2(w.x), qa[s][2 + x] = half2(w.y);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) q_frag(qa[s], s);
-    }
-    float kd = 1.f, vd = 1.f;
-    if constexpr (FP8) {
-      kd = p.k_descale * (p.k_descale_heads ? __ldg(p.k_descale_heads + pc.h) : 1.f);
-      vd = p.v_descale * (p.v_descale_heads ? __ldg(p.v_descale_heads + pc.h) : 1.f);
-    }
-    const float scale2 = p.scale * kLog2e;
-    float o[kTilesD][4];
-#pragma unroll
-    for (int t = 0; t < kTilesD; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-    // Scores (rows grp, grp + 8; keys 2 quad + {0, 1} of two groups of 8) to
-    // weights; updates m, l and rescales o where a maximum moved.
-    auto softmax = [&](float (&s)[2][4]) {
+    // The same in f16 and in the order of d in which a thread finds 16 of an
+    // e4m3 key's values in one load: for k-step s, k = 2 quad + {0, 1} and
+    // 2 quad + 8 + {0, 1} are the 4 values from d on.
+    auto q_frag8 = [&](uint32_t (&a)[4], int mt, int s) {
+      const int d = (s >> 2) * 64 + quad * 16 + (s & 3) * 4;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float top = fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        top = fmaxf(top, m[x]);
-        if (__any_sync(0xffffffffu, top != m[x])) {
-          const float a = top == -INFINITY ? 1.f : attn_sm100::ex2(m[x] - top);
-          l[x] *= a;
-#pragma unroll
-          for (int t = 0; t < kTilesD; ++t) o[t][2 * x] *= a, o[t][2 * x + 1] *= a;
-          m[x] = top;
+        const int r = 16 * mt + grp + 8 * x;
+        const uint2 w = *reinterpret_cast<const uint2*>(s_q + r * D * 2 + (((d >> 3) ^ (r & 7)) * 16) + (d & 7) * 2);
+        if constexpr (F16) {
+          a[x] = w.x, a[2 + x] = w.y;
+        } else {
+          const float inv = 1.f / q_unit[r];  // a power of two
+          a[x] = attn_sm100::pack_f16(__uint_as_float(w.x << 16) * inv, __uint_as_float(w.x & 0xffff0000u) * inv);
+          a[2 + x] = attn_sm100::pack_f16(__uint_as_float(w.y << 16) * inv, __uint_as_float(w.y & 0xffff0000u) * inv);
         }
-        const float sub = (top == -INFINITY ? 0.f : top) - C::kShift;
-        float add = 0.f;
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            s[g][2 * x + e] = attn_sm100::ex2(s[g][2 * x + e] - sub);
-            add += s[g][2 * x + e];
-          }
-        l[x] += add;
       }
     };
+    uint32_t qa[kHoldQ ? kSteps : 1][4];
+    if constexpr (kHoldQ) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if constexpr (FP8) q_frag8(qa[s], 0, s);
+        else q_frag(qa[s], 0, s);
+      }
+    }
+    float kd = scale2, vd = 1.f;
+    if constexpr (FP8) {
+      kd *= p.k_descale * (p.k_descale_heads ? __ldg(p.k_descale_heads + pc.h) : 1.f);
+      vd = p.v_descale * (p.v_descale_heads ? __ldg(p.v_descale_heads + pc.h) : 1.f);
+    }
+    float o[MT][kTilesD][4];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt][0] = m[mt][1] = -INFINITY, l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < kTilesD; ++t) o[mt][t][0] = o[mt][t][1] = o[mt][t][2] = o[mt][t][3] = 0.f;
+    }
     bool scaled = !FP8;  // o is in units of the cached values until the new ones come
 
     for (int k = pc.k0; k < pc.k1; ++k, ++n) {
-      const int st = static_cast<int>(n % C::kStages);
+      const int st = n % C::kStages;
       const uint32_t u = static_cast<uint32_t>(n / C::kStages);
-      if (ok) ok = __all_sync(0xffffffffu, attn_sm100::mbar_wait_bounded(&full[st], u & 1u, &abort_flag, p.status, kWaitLimitNs));
+      if (ok)
+        ok = __all_sync(0xffffffffu, attn_sm100::mbar_wait_bounded(&full[st], u & 1u, &abort_flag, p.status,
+                                                                   kWaitLimitNs));
       const uint32_t ks = s_ring + st * 2 * C::kTile, vs = ks + C::kTile;
       const bool cached = k < pc.cached;
       const int first = cached ? k << split.keys_shift : (k - pc.cached) << split.new_shift;
       const int here = cached ? min(1 << split.keys_shift, pc.r.held - first)
                               : min(1 << split.new_shift, pc.r.count - first);
-      const int kb = warp * 16;  // this warp's keys of the tile
-      if (kb < here && ok) {
-        const int seg_shift = cached ? min(p.page_shift, split.keys_shift) : split.new_shift;
-        const int seg = kb >> seg_shift, r0 = kb & ((1 << seg_shift) - 1);
-        float s[2][4] = {};
+      const int seg_shift = cached ? min(p.page_shift, split.keys_shift) : split.new_shift;
+      // This warp's groups of 16 keys, NG at a time (of a new tile: one).
+      const int kb_end = cached ? 16 * C::kGroups * (warp + 1) : 16 * (warp + 1);
+      for (int kb = cached ? 16 * C::kGroups * warp : 16 * warp; kb < min(kb_end, here) && ok; kb += 16 * NG) {
+        float s[NG][MT][2][4];
+        uint32_t kbase[NG], vbase[NG];  // of the group's page segment
+        int r0[NG];                     // its first row there
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const int j = kb + 16 * g, seg = j >> seg_shift;
+          r0[g] = j & ((1 << seg_shift) - 1);
+          const uint32_t off = seg * ((cached ? C::kRowBytes : C::kNewRowBytes) << seg_shift);
+          kbase[g] = ks + off, vbase[g] = vs + off;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[g][mt][h][0] = s[g][mt][h][1] = s[g][mt][h][2] = s[g][mt][h][3] = 0.f;
+        }
         if (FP8 && cached) {
-          // Key r (row of 128 bytes): thread quad loads 16 values at 16 quad and
-          // 16 at 64 + 16 quad; k-step s takes 4 of them, for k = 2 quad + {0, 1}
-          // and 2 quad + 8 + {0, 1}: q_frag's order.
+          // Key r (a row of 128 bytes): thread quad loads 16 values at 16 quad
+          // and 16 at 64 + 16 quad (see q_frag8).
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const int r = r0 + 8 * g + grp;
-            const uint32_t base = ks + seg * (C::kRowBytes << seg_shift) + r * 128;
+          for (int c = 0; c < 2; ++c) {
+            uint4 w[NG][2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const uint4 w = lds128(base + (((quad + 4 * c) ^ (r & 7)) * 16));
-              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            for (int g = 0; g < NG; ++g)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                mma16816<true>(s[g], qa[4 * c + e], f16_of_e4m3(ww[e]), f16_of_e4m3(ww[e] >> 16));
+              for (int h = 0; h < 2; ++h) {
+                const int r = r0[g] + 8 * h + grp;
+                w[g][h] = lds128(kbase[g] + r * 128 + (((quad + 4 * c) ^ (r & 7)) * 16));
+              }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                uint32_t a[4];
+                if constexpr (kHoldQ) a[0] = qa[4 * c + e][0], a[1] = qa[4 * c + e][1], a[2] = qa[4 * c + e][2], a[3] = qa[4 * c + e][3];
+                else q_frag8(a, mt, 4 * c + e);
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const uint32_t ww = e == 0 ? w[g][h].x : e == 1 ? w[g][h].y : e == 2 ? w[g][h].z : w[g][h].w;
+                    mma16816<true>(s[g][mt][h], a, f16_of_e4m3(ww), f16_of_e4m3(ww >> 16));
+                  }
+              }
             }
           }
         } else {
-          const uint32_t base = ks + seg * (C::kNewRowBytes << seg_shift);
-          const int r = r0 + (lane & 7) + 8 * (lane >> 4);
 #pragma unroll
           for (int x = 0; x < kSteps; ++x) {
             const int chunk = 2 * x + ((lane >> 3) & 1);
-            uint32_t b[4];
-            ldmatrix4(b, base + (chunk >> 3) * (128 << seg_shift) + r * 128 + (((chunk & 7) ^ (r & 7)) * 16));
-            if constexpr (FP8) {
-              uint32_t a[4];
-              q_frag(a, x);
-              mma16816<F16>(s[0], a, b[0], b[1]);
-              mma16816<F16>(s[1], a, b[2], b[3]);
-            } else {
-              mma16816<F16>(s[0], qa[x], b[0], b[1]);
-              mma16816<F16>(s[1], qa[x], b[2], b[3]);
+#pragma unroll
+            for (int g = 0; g < (FP8 ? 1 : NG); ++g) {
+              const int r = r0[g] + (lane & 7) + 8 * (lane >> 4);
+              uint32_t b[4];
+              ldmatrix4(b, kbase[g] + (chunk >> 3) * (128 << seg_shift) + r * 128 + (((chunk & 7) ^ (r & 7)) * 16));
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                uint32_t a[4];
+                if constexpr (kHoldQ && !FP8) a[0] = qa[x][0], a[1] = qa[x][1], a[2] = qa[x][2], a[3] = qa[x][3];
+                else q_frag(a, mt, x);
+                mma16816<F16>(s[g][mt][0], a, b[0], b[1]);
+                mma16816<F16>(s[g][mt][1], a, b[2], b[3]);
+              }
             }
           }
         }
         // Scale, then the mask (selected after the scale: what a masked key's
-        // score was does not matter).
-        const float f0 = FP8 && cached ? scale2 * kd * unit[0] : scale2;
-        const float f1 = FP8 && cached ? scale2 * kd * unit[1] : scale2;
+        // score was does not matter), then weights: rows grp, grp + 8 of each
+        // 16; keys 2 quad + {0, 1} of each 8.  All rows' maxima first, so that
+        // their exchanges overlap, and one vote on whether any moved.
+        const bool tail = kb + 16 * NG > here;
+        float top[MT][2];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          s[g][0] *= f0, s[g][1] *= f0, s[g][2] *= f1, s[g][3] *= f1;
-        }
-        if (cached) {
-          if (kb + 16 > here) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (kb + 8 * g + 2 * quad + (e & 1) >= here) s[g][e] = -INFINITY;
-          }
-        } else {
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int i = (pc.rt * kMmaRows + grp + 8 * x) / p.group;  // token of the request
-            const bool live = grp + 8 * x < rows;
-            const uint8_t* mrow = p.mask + static_cast<int64_t>(pc.r.first + (live ? i : 0)) * p.mask_stride;
+            const float f = FP8 && cached ? (F16 ? kd : kd * q_unit[16 * mt + grp + 8 * x]) : scale2;
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
+            for (int g = 0; g < NG; ++g)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int j = kb + 8 * g + 2 * quad + e;
-                bool hide = j >= here || !live;
-                if (!hide) hide = p.mask ? mrow[first + j] != 0 : first + j > i;
-                if (hide) s[g][2 * x + e] = -INFINITY;
-              }
+              for (int h = 0; h < 2; ++h) s[g][mt][h][2 * x] *= f, s[g][mt][h][2 * x + 1] *= f;
           }
+        if (!cached) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int r = 16 * mt + grp + 8 * x;
+              const bool live = r < rows;
+              const int i = (row0 + r) / p.group;  // token of the request
+              const uint8_t* const mrow =
+                  p.mask + static_cast<int64_t>(pc.r.first + (live ? i : 0)) * p.mask_stride + first;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int j = kb + 8 * h + 2 * quad + e;
+                  bool hide = j >= here || !live;
+                  if (!hide) hide = p.mask ? mrow[j] != 0 : first + j > i;
+                  if (hide) s[0][mt][h][2 * x + e] = -INFINITY;
+#pragma unroll
+                  for (int g = 1; g < NG; ++g) s[g][mt][h][2 * x + e] = -INFINITY;
+                }
+            }
+        } else if (tail) {
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (kb + 16 * g + 8 * h + 2 * quad + e >= here) {
+#pragma unroll
+                  for (int mt = 0; mt < MT; ++mt) s[g][mt][h][e] = s[g][mt][h][2 + e] = -INFINITY;
+                }
         }
-        softmax(s);
-        // Weights of keys that are not there are 0; their values are made 0 too
-        // (0 times what lies in memory there need not be 0).
-        const bool tail = kb + 16 > here;
-        uint32_t live0 = 0xffffffffu, live1 = 0xffffffffu;
-        if (tail) {
-          const int j = kb + 2 * quad;
-          live0 = (j < here ? 0xffffu : 0u) | (j + 1 < here ? 0xffff0000u : 0u);
-          live1 = (j + 8 < here ? 0xffffu : 0u) | (j + 9 < here ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            top[mt][x] = m[mt][x];
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+              top[mt][x] = fmaxf(top[mt][x], fmaxf(fmaxf(s[g][mt][0][2 * x], s[g][mt][0][2 * x + 1]),
+                                                   fmaxf(s[g][mt][1][2 * x], s[g][mt][1][2 * x + 1])));
+          }
+#pragma unroll
+        for (int d = 1; d <= 2; d *= 2)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              top[mt][x] = fmaxf(top[mt][x], __shfl_xor_sync(0xffffffffu, top[mt][x], d));
+        bool moved = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) moved = moved || top[mt][0] != m[mt][0] || top[mt][1] != m[mt][1];
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float a = top[mt][x] == -INFINITY ? 1.f : attn_sm100::ex2(m[mt][x] - top[mt][x]);
+              l[mt][x] *= a;
+#pragma unroll
+              for (int t = 0; t < kTilesD; ++t) o[mt][t][2 * x] *= a, o[mt][t][2 * x + 1] *= a;
+              m[mt][x] = top[mt][x];
+            }
         }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float sub = (top[mt][x] == -INFINITY ? 0.f : top[mt][x]) - C::kShift;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float& v = s[g][mt][h][2 * x + e];
+                  v = attn_sm100::ex2(v - sub);
+                  l[mt][x] += v;
+                }
+          }
         if (!cached && !scaled) {
 #pragma unroll
-          for (int t = 0; t < kTilesD; ++t)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[t][e] *= vd;
+            for (int t = 0; t < kTilesD; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[mt][t][e] *= vd;
           scaled = true;
         }
-        if constexpr (FP8) {
-          // Values: thread group grp loads 16 of each of its four keys (2 quad,
-          // + 1, + 8, + 9) at 16 grp; n-tile t is d = 16 n + t, n = 0..7.
-          if (cached) {
-            uint32_t a[4] = {pack2<true>(s[0][0], s[0][1]), pack2<true>(s[0][2], s[0][3]),
-                             pack2<true>(s[1][0], s[1][1]), pack2<true>(s[1][2], s[1][3])};
-            uint32_t w[4][4];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          if (FP8 && !cached && g > 0) break;
+          uint32_t a[MT][4], rest[MT][4];
+          const bool p16 = F16 || (FP8 && cached);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const int r = r0 + 2 * quad + (y & 1) + 8 * (y >> 1);
-              const uint4 v = lds128(vs + seg * (C::kRowBytes << seg_shift) + r * 128 + ((grp ^ (r & 7)) * 16));
-              w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
+              const float x0 = s[g][mt][y >> 1][2 * (y & 1)], x1 = s[g][mt][y >> 1][2 * (y & 1) + 1];
+              a[mt][y] = p16 ? pack2<true>(x0, x1) : pack2<false>(x0, x1);
+              if constexpr (C::kTwoParts)
+                rest[mt][y] = pack2<false>(x0 - __uint_as_float(a[mt][y] << 16),
+                                           x1 - __uint_as_float(a[mt][y] & 0xffff0000u));
             }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-#pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                const uint32_t lo = __byte_perm(w[0][c], w[1][c], z ? 0x7362 : 0x5140);
-                const uint32_t hi = __byte_perm(w[2][c], w[3][c], z ? 0x7362 : 0x5140);
-                mma16816<true>(o[4 * c + 2 * z], a, f16_of_e4m3(lo) & live0, f16_of_e4m3(hi) & live1);
-                mma16816<true>(o[4 * c + 2 * z + 1], a, f16_of_e4m3(lo >> 16) & live0, f16_of_e4m3(hi >> 16) & live1);
-              }
-            }
-          } else {
-            uint32_t a[4] = {pack2<F16>(s[0][0], s[0][1]), pack2<F16>(s[0][2], s[0][3]),
-                             pack2<F16>(s[1][0], s[1][1]), pack2<F16>(s[1][2], s[1][3])};
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {  // 8 of the 16 values at a time
+          // The values of keys that are not there are made 0 (their weights
+          // are 0, but 0 times what lies in memory there need not be 0).
+          const int j0 = kb + 16 * g + 2 * quad;
+          if constexpr (FP8) {
+            // Thread group grp loads 16 values of each of its four keys (2 quad,
+            // + 1, + 8, + 9) at 16 grp; n-tile t is d = 16 n + t, n = 0..7.
+            if (cached) {
               uint32_t w[4][4];
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                const int r = r0 + 2 * quad + (y & 1) + 8 * (y >> 1), chunk = 2 * grp + c;
-                const uint4 v = lds128(vs + (chunk >> 3) * (128 << seg_shift) + r * 128 + (((chunk & 7) ^ (r & 7)) * 16));
+                const int r = r0[g] + 2 * quad + (y & 1) + 8 * (y >> 1);
+                const uint4 v = lds128(vbase[g] + r * 128 + ((grp ^ (r & 7)) * 16));
                 w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
               }
+              if (tail) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-                mma16816<F16>(o[8 * c + e], a, __byte_perm(w[0][e >> 1], w[1][e >> 1], sel) & live0,
-                              __byte_perm(w[2][e >> 1], w[3][e >> 1], sel) & live1);
+                for (int y = 0; y < 4; ++y)
+                  if (j0 + (y & 1) + 8 * (y >> 1) >= here) w[y][0] = w[y][1] = w[y][2] = w[y][3] = 0u;
+              }
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                  const uint32_t lo = __byte_perm(w[0][c], w[1][c], z ? 0x7362 : 0x5140);
+                  const uint32_t hi = __byte_perm(w[2][c], w[3][c], z ? 0x7362 : 0x5140);
+                  const uint32_t b0 = f16_of_e4m3(lo), b1 = f16_of_e4m3(hi);
+                  const uint32_t b2 = f16_of_e4m3(lo >> 16), b3 = f16_of_e4m3(hi >> 16);
+#pragma unroll
+                  for (int mt = 0; mt < MT; ++mt) {
+                    mma16816<true>(o[mt][4 * c + 2 * z], a[mt], b0, b1);
+                    mma16816<true>(o[mt][4 * c + 2 * z + 1], a[mt], b2, b3);
+                  }
+                }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {  // 8 of the 16 values at a time
+                uint32_t w[4][4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const int r = r0[g] + 2 * quad + (y & 1) + 8 * (y >> 1), chunk = 2 * grp + c;
+                  const uint4 v = lds128(vbase[g] + (chunk >> 3) * (128 << seg_shift) + r * 128 +
+                                         (((chunk & 7) ^ (r & 7)) * 16));
+                  w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
+                  if (j0 + (y & 1) + 8 * (y >> 1) >= here) w[y][0] = w[y][1] = w[y][2] = w[y][3] = 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+                  const uint32_t b0 = __byte_perm(w[0][e >> 1], w[1][e >> 1], sel);
+                  const uint32_t b1 = __byte_perm(w[2][e >> 1], w[3][e >> 1], sel);
+#pragma unroll
+                  for (int mt = 0; mt < MT; ++mt) mma16816<F16>(o[mt][8 * c + e], a[mt], b0, b1);
+                }
               }
             }
-          }
-        } else {
-          uint32_t a[4], rest[4];
+          } else {
+            const int r = r0[g] + (lane & 7) + 8 * ((lane >> 3) & 1);
+            const uint32_t live0 = (j0 < here ? 0xffffu : 0u) | (j0 + 1 < here ? 0xffff0000u : 0u);
+            const uint32_t live1 = (j0 + 8 < here ? 0xffffu : 0u) | (j0 + 9 < here ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float x0 = s[y >> 1][2 * (y & 1)], x1 = s[y >> 1][2 * (y & 1) + 1];
-            a[y] = pack2<F16>(x0, x1);
-            if constexpr (!F16)
-              rest[y] = pack2<false>(x0 - __uint_as_float(a[y] << 16), x1 - __uint_as_float(a[y] & 0xffff0000u));
-          }
-          const uint32_t base = vs + seg * (C::kNewRowBytes << seg_shift);
-          const int r = r0 + (lane & 7) + 8 * ((lane >> 3) & 1);
+            for (int t = 0; t < kTilesD / 2; ++t) {
+              const int chunk = 2 * t + (lane >> 4);
+              uint32_t b[4];
+              ldmatrix4t(b, vbase[g] + (chunk >> 3) * (128 << seg_shift) + r * 128 + (((chunk & 7) ^ (r & 7)) * 16));
+              if (tail) b[0] &= live0, b[1] &= live1, b[2] &= live0, b[3] &= live1;
 #pragma unroll
-          for (int t = 0; t < kTilesD / 2; ++t) {
-            const int chunk = 2 * t + (lane >> 4);
-            uint32_t b[4];
-            ldmatrix4t(b, base + (chunk >> 3) * (128 << seg_shift) + r * 128 + (((chunk & 7) ^ (r & 7)) * 16));
-            if (tail) b[0] &= live0, b[1] &= live1, b[2] &= live0, b[3] &= live1;
-            mma16816<F16>(o[2 * t], a, b[0], b[1]);
-            mma16816<F16>(o[2 * t + 1], a, b[2], b[3]);
-            if constexpr (!F16) {
-              mma16816<F16>(o[2 * t], rest, b[0], b[1]);
-              mma16816<F16>(o[2 * t + 1], rest, b[2], b[3]);
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16816<F16>(o[mt][2 * t], a[mt], b[0], b[1]);
+                mma16816<F16>(o[mt][2 * t + 1], a[mt], b[2], b[3]);
+                if constexpr (C::kTwoParts) {
+                  mma16816<F16>(o[mt][2 * t], rest[mt], b[0], b[1]);
+                  mma16816<F16>(o[mt][2 * t + 1], rest[mt], b[2], b[3]);
+                }
+              }
             }
           }
         }
@@ -511,95 +622,101 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
     }
 
     // ---------------------------------------------------------- a piece ends
-    if (!scaled) {
-#pragma unroll
-      for (int t = 0; t < kTilesD; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[t][e] *= vd;
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (quad == 0) warp_m[warp][grp + 8 * x] = m[x], warp_l[warp][grp + 8 * x] = l[x];
-    }
-    readers_sync();
-    float factor[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kMmaWarps; ++w) top = fmaxf(top, warp_m[w][grp + 8 * x]);
-      factor[x] = top == -INFINITY ? 0.f : attn_sm100::ex2(m[x] - top);
-    }
-    // The row that this thread writes: tid / 8, columns 4 (tid % 8) of 32.
-    const int wr = tid >> 3, wc = (tid & 7) * 4;
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kMmaWarps; ++w) top = fmaxf(top, warp_m[w][wr]);
-    if (top != -INFINITY) {
-#pragma unroll
-      for (int w = 0; w < kMmaWarps; ++w) sum += attn_sm100::ex2(warp_m[w][wr] - top) * warp_l[w][wr];
-    }
     const bool whole = pc.k0 == 0 && pc.k1 == pc.tiles;
-    const int slot = 2 * blockIdx.x + (share.lo - (pc.k1 - pc.k0) == share_lo ? 0 : 1);
-    int token, head;
-    row_of(wr, token, head);
+    const int slot = 2 * sid + (share.lo - (pc.k1 - pc.k0) == share_lo ? 0 : 1);
 #pragma unroll
-    for (int c0 = 0; c0 < D; c0 += 32) {
-      // The accumulators of columns c0 .. c0 + 31 (an e4m3 cache: n-tile t is
-      // columns 16 n + t, so they are one thread of each quad's).
-      if constexpr (FP8) {
-        if (quad == c0 / 32) {
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int t = 0; t < kTilesD; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s_join[(warp * kMmaRows + grp + 8 * (e >> 1)) * 32 + 16 * (e & 1) + t] = o[t][e] * factor[e >> 1];
-        }
-        __syncwarp();
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            *reinterpret_cast<float2*>(s_join + (warp * kMmaRows + grp + 8 * x) * 32 + 8 * t + 2 * quad) =
-                make_float2(o[c0 / 8 + t][2 * x] * factor[x], o[c0 / 8 + t][2 * x + 1] * factor[x]);
+      for (int x = 0; x < 2; ++x) {
+        l[mt][x] += __shfl_xor_sync(0xffffffffu, l[mt][x], 1);
+        l[mt][x] += __shfl_xor_sync(0xffffffffu, l[mt][x], 2);
+        if (quad == 0) warp_m[warp][16 * mt + grp + 8 * x] = m[mt][x], warp_l[warp][16 * mt + grp + 8 * x] = l[mt][x];
       }
-      readers_sync();
-      if (wr < rows) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    readers_sync(team);
 #pragma unroll
-        for (int w = 0; w < kMmaWarps; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(s_join + (w * kMmaRows + wr) * 32 + wc);
-          x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-        }
-        if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          uint2 w = make_uint2(pack2<F16>(x.x * inv, x.y * inv), pack2<F16>(x.z * inv, x.w * inv));
-          *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + c0 + wc) = w;
+    for (int mt = 0; mt < MT; ++mt) {
+      float factor[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kMmaWarps; ++w) top = fmaxf(top, warp_m[w][16 * mt + grp + 8 * x]);
+        factor[x] = top == -INFINITY ? 0.f : attn_sm100::ex2(m[mt][x] - top);
+        if (!scaled) factor[x] *= vd;
+      }
+      // The row that this thread writes, and its four columns of kJoinCols.
+      constexpr int kPer = C::kJoinCols / 4;
+      const int wr = 16 * mt + (tid / kPer & 15), wc = (tid % kPer) * 4;
+      const bool writes = tid < 16 * kPer && wr < rows;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kMmaWarps; ++w) top = fmaxf(top, warp_m[w][wr]);
+      if (top != -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < kMmaWarps; ++w) sum += attn_sm100::ex2(warp_m[w][wr] - top) * warp_l[w][wr];
+      }
+      const int at = row0 + wr;
+      const int token = pc.r.first + at / p.group, head = pc.h * p.group + at % p.group;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += C::kJoinCols) {
+        float* const mine = s_join + (warp * 16 + grp) * C::kJoinCols;  // + 8 rows
+        // The accumulators of columns c0 .. c0 + kJoinCols - 1 (an e4m3 cache:
+        // n-tile t is columns 16 n + t, so they are one thread's of each quad).
+        if constexpr (FP8) {
+          if (quad == c0 / 32) {
+#pragma unroll
+            for (int t = 0; t < kTilesD; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (C::kJoinCols == 32)
+                  mine[(e >> 1) * 8 * C::kJoinCols + 16 * (e & 1) + t] = o[mt][t][e] * factor[e >> 1];
+                else if ((e & 1) == (c0 / 16 & 1))
+                  mine[(e >> 1) * 8 * C::kJoinCols + t] = o[mt][t][e] * factor[e >> 1];
+              }
+          }
         } else {
-          scratch.o[(static_cast<int64_t>(slot) * kMmaRows + wr) * (D / 4) + (c0 + wc) / 4] = x;
+#pragma unroll
+          for (int t = 0; t < C::kJoinCols / 8; ++t)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              *reinterpret_cast<float2*>(mine + x * 8 * C::kJoinCols + 8 * t + 2 * quad) =
+                  make_float2(o[mt][c0 / 8 + t][2 * x] * factor[x], o[mt][c0 / 8 + t][2 * x + 1] * factor[x]);
+        }
+        readers_sync(team);
+        if (writes) {
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kMmaWarps; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(s_join + (w * 16 + (wr & 15)) * C::kJoinCols + wc);
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+          }
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + c0 + wc) =
+                make_uint2(pack2<F16>(x.x * inv, x.y * inv), pack2<F16>(x.z * inv, x.w * inv));
+          } else {
+            scratch.o[(static_cast<int64_t>(slot) * C::kRows + wr) * (D / 4) + (c0 + wc) / 4] = x;
+          }
+        }
+        readers_sync(team);
+      }
+      if (writes && wc == 0) {
+        if (whole) {
+          if (p.lse)
+            p.lse[static_cast<int64_t>(token) * p.Hq + head] =
+                sum == 0.f ? -INFINITY : (top - C::kShift + log2f(sum)) * kLn2;
+        } else {
+          scratch.m[slot * C::kRows + wr] = top;
+          scratch.l[slot * C::kRows + wr] = sum;
         }
       }
-      readers_sync();
     }
-    if ((tid & 7) == 0 && wr < rows) {
-      if (whole) {
-        if (p.lse)
-          p.lse[static_cast<int64_t>(token) * p.Hq + head] =
-              sum == 0.f ? -INFINITY : (top - C::kShift + log2f(sum)) * kLn2;
-      } else {
-        scratch.m[slot * kMmaRows + wr] = top;
-        scratch.l[slot * kMmaRows + wr] = sum;
-      }
-    }
-    if (!whole && pc.k0 == 0 && tid == 0) scratch.record[blockIdx.x] = make_record(p, split, share, pc, slot);
+    if (!whole && pc.k0 == 0 && tid == 0) scratch.record[sid] = make_record(p, split, share, pc, sid, slot);
   }
 }
 
 // Joins the pieces of the items that were cut: block (c, y) takes `rows_each`
-// query rows of the cut item that begins in block c of the first kernel, if
+// query rows of the cut item that begins in share c of the first kernel, if
 // any.  What bounds it is latency, a record and then everything else at once:
 // a thread has four columns of a row and every G-th piece of the item, brought
 // to one maximum as it goes; the G parts meet in shared memory.  The order of
@@ -607,7 +724,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2)
 // time.
 constexpr int kJoinThreads = 256;
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads)
     tree_mma_join(const __grid_constant__ Params p, const Scratch scratch, const int rows_each, const float shift) {
   constexpr bool F16 = std::is_same<T, __half>::value;
@@ -638,9 +755,9 @@ __global__ void __launch_bounds__(kJoinThreads)
           m[x] = -INFINITY, l[x] = 0.f, y[x] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (i < n) {
             const int s = i == 0 ? rec.slot : 2 * (c + i);
-            m[x] = scratch.m[s * kMmaRows + row];
-            l[x] = scratch.l[s * kMmaRows + row];
-            y[x] = scratch.o[(static_cast<int64_t>(s) * kMmaRows + row) * kCols + col];
+            m[x] = scratch.m[s * ROWS + row];
+            l[x] = scratch.l[s * ROWS + row];
+            y[x] = scratch.o[(static_cast<int64_t>(s) * ROWS + row) * kCols + col];
           }
         }
         const float high = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);

@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_release();
   if (tid == 0) scratch.record[blockIdx.x].pieces = 0;
   tc_fence_before();
-  Share share = find_share(p, split, min_units);
+  Share share = find_share<1>(p, split, min_units, 0);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           const int rec = 2 * blockIdx.x + (lo == share_lo ? 0 : 1);
           if (more && pc.k0 == 0 && pc.k1 < pc.tiles)
-            scratch.record[blockIdx.x] = make_record(p, split, share, pc, rec);
+            scratch.record[blockIdx.x] = make_record(p, split, share, pc, blockIdx.x, rec);
           if (more) jobs[i] = make_job(p, split, tiles, pc, rec);
           else jobs[i].b = -1;
           mbar_arrive(&job_full[i]);

@@ -418,10 +418,10 @@ int make_key_maps(KeyMaps* m, const AttnTree& d, int box, int new_box, bool all_
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Scratch for the cut items of a launch of `blocks` blocks.
-int tree_scratch(attn_tree::Scratch* out, void** base, int blocks, int rows, int D, cudaStream_t s) {
-  const size_t slots = 2 * static_cast<size_t>(blocks);
-  const size_t rec = round256(blocks * sizeof(attn_tree::Record)), ml = round256(slots * rows * sizeof(float));
+// Scratch for the cut items of a launch whose work is cut into `shares`.
+int tree_scratch(attn_tree::Scratch* out, void** base, int shares, int rows, int D, cudaStream_t s) {
+  const size_t slots = 2 * static_cast<size_t>(shares);
+  const size_t rec = round256(shares * sizeof(attn_tree::Record)), ml = round256(slots * rows * sizeof(float));
   const cudaError_t e = rt_host::scratch(base, rec + 2 * ml + slots * rows * D * sizeof(float), s);
   if (e != cudaSuccess) return cuda_fail(e, "stream-ordered scratch (cut items)");
   char* at = static_cast<char*>(*base);
@@ -451,13 +451,18 @@ cudaError_t launch_early(void (*kern)(K...), dim3 grid, int threads, size_t smem
 
 // Both kernels keep the SM's memory split as the first one needs it: a change
 // of it between them would drain the SM.
+// `pool`: what the kernel's warpgroups divide among themselves has to fit in
+// the registers that a block is launched with, or the raise would wait forever.
 template <typename K, typename J>
-cudaError_t prepare_kernels(K kern, J join, size_t smem) {
+cudaError_t prepare_kernels(K kern, J join, size_t smem, int threads, int pool) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(join, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  cudaFuncAttributes fa{};
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, kern);
+  if (e == cudaSuccess && fa.numRegs * threads < pool) e = cudaErrorLaunchOutOfResources;
   return e;
 }
 
@@ -467,43 +472,55 @@ int pow2_shift(int64_t n, int lo, int hi) {
   return s;
 }
 
-template <typename T, typename TC, int D>
+template <typename T, typename TC, int D, int MT>
 int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, const rt_host::Device& dev, cudaStream_t s) {
-  using C = attn_tree::MmaCfg<T, TC, D>;
-  constexpr int kRows = attn_tree::kMmaRows;
-  auto kern = attn_tree::tree_mma_kernel<T, TC, D>;
+  using C = attn_tree::MmaCfg<T, TC, D, MT>;
+  auto kern = attn_tree::tree_mma_kernel<T, TC, D, MT>;
+  auto join = attn_tree::tree_mma_join<T, D, C::kRows>;
   static std::once_flag once[64];
   static cudaError_t attr[64];
   std::call_once(once[dev.index], [&] {
-    attr[dev.index] = prepare_kernels(kern, attn_tree::tree_mma_join<T, D>, C::kSmem);
+    attr[dev.index] = prepare_kernels(kern, join, C::kSmem, attn_tree::kMmaThreads, attn_tree::kMmaRegPool);
   });
-  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "cudaFuncSetAttribute");
+  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "set-up of a kernel");
   attn_tree::Split split;
-  split.rows = kRows;
-  split.keys_shift = 6;
-  split.new_shift = pow2_shift(p.max_new, 3, C::kNewKeys == 64 ? 6 : 5);
+  split.rows = C::kRows;
+  split.keys_shift = C::kKeysShift;
+  split.new_shift = pow2_shift(p.max_new, 3, C::kNewShift);
   KeyMaps m;
-  int rc = make_key_maps(&m, d, std::min(1 << p.page_shift, attn_tree::kMmaKeys), 1 << split.new_shift, true);
+  int rc = make_key_maps(&m, d, std::min(1 << p.page_shift, 1 << C::kKeysShift), 1 << split.new_shift, true);
   if (rc != ATTN_OK) return rc;
-  const int blocks = 2 * dev.sms;
-  const int rows = static_cast<int>(std::min<int64_t>(kRows, static_cast<int64_t>(p.max_new) * p.group));
+  const int shares = attn_tree::kMmaTeams * dev.sms;
+  const int rows = static_cast<int>(std::min<int64_t>(C::kRows, static_cast<int64_t>(p.max_new) * p.group));
   attn_tree::Scratch sc{};
   void* base = nullptr;
-  if ((rc = tree_scratch(&sc, &base, blocks, kRows, D, s)) != ATTN_OK) return rc;
-  cudaError_t e = launch_early(kern, dim3(blocks), attn_tree::kMmaThreads, C::kSmem, s, m.kc, m.vc, m.kn, m.vn, p,
+  if ((rc = tree_scratch(&sc, &base, shares, C::kRows, D, s)) != ATTN_OK) return rc;
+  cudaError_t e = launch_early(kern, dim3(dev.sms), attn_tree::kMmaThreads, C::kSmem, s, m.kc, m.vc, m.kn, m.vn, p,
                                split, sc, 1);
   if (e == cudaSuccess) {
     // Rows of a join block: about twice the blocks that fit at once; more
     // would come too late to hide their start.
     const int at_once = dev.sms * (2048 / attn_tree::kJoinThreads);
-    const int each = std::max(1, blocks * rows / (2 * at_once));
-    e = launch_early(attn_tree::tree_mma_join<T, D>, dim3(blocks, (rows + each - 1) / each), attn_tree::kJoinThreads, 0,
-                     s, p, sc, each, C::kShift);
+    const int each = std::max(1, shares * rows / (2 * at_once));
+    e = launch_early(join, dim3(shares, (rows + each - 1) / each), attn_tree::kJoinThreads, 0, s, p, sc, each,
+                     C::kShift);
   }
   cudaFreeAsync(base, s);
   if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
   rt_host::count_launches(2);
   return ATTN_OK;
+}
+
+// The kernel for few rows, with as many 16-row tiles as the rows of a request
+// need, up to 2 (at D = 64: 4).
+template <typename T, typename TC, int D>
+int launch_tree_few(const AttnTree& d, const attn_tree::Params& p, int64_t rows, const rt_host::Device& dev,
+                    cudaStream_t s) {
+  if (rows <= 16) return launch_tree_mma<T, TC, D, 1>(d, p, dev, s);
+  if constexpr (D == 64) {
+    if (rows > 32) return launch_tree_mma<T, TC, D, 4>(d, p, dev, s);
+  }
+  return launch_tree_mma<T, TC, D, 2>(d, p, dev, s);
 }
 
 template <typename T, int D>
@@ -512,18 +529,11 @@ int launch_tree_tc(const AttnTree& d, const attn_tree::Params& p, const rt_host:
   auto kern = attn_tree::tc::tree_tc_kernel<T, D>;
   static std::once_flag once[64];
   static cudaError_t attr[64];
-  static int regs[64];
   std::call_once(once[dev.index], [&] {
-    cudaFuncAttributes fa{};
-    attr[dev.index] = prepare_kernels(kern, attn_tree::tc::tree_tc_join<T, D>, C::kSmem);
-    if (attr[dev.index] == cudaSuccess) attr[dev.index] = cudaFuncGetAttributes(&fa, kern);
-    regs[dev.index] = fa.numRegs;
+    attr[dev.index] = prepare_kernels(kern, attn_tree::tc::tree_tc_join<T, D>, C::kSmem, attn_tree::tc::kThreads,
+                                      attn_tree::tc::kRegPool);
   });
-  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "cudaFuncSetAttribute");
-  // The warpgroups' register split has to fit what a block is launched with.
-  if (regs[dev.index] * attn_tree::tc::kThreads < attn_tree::tc::kRegPool)
-    return fail(ATTN_ERR_UNSUPPORTED, "kernel built with %d registers per thread; the register split needs %d",
-                regs[dev.index], attn_tree::tc::kRegPool / attn_tree::tc::kThreads);
+  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "set-up of a kernel");
   attn_tree::tc::Tiles tiles;
   tiles.box = std::max(1, std::min(attn_tree::tc::kTileRows / p.group, p.max_new));
   tiles.rows = tiles.box * p.group;
@@ -599,16 +609,17 @@ int run(const AttnTree& d, cudaStream_t s) {
   using N = __nv_bfloat16;
   using E = __nv_fp8_e4m3;
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
-  if (!fp8 && static_cast<int64_t>(p.max_new) * p.group > attn_tree::kMmaRows) {
+  const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
+  if (!fp8 && rows > (d.D == 64 ? 64 : 32)) {
     auto launch = d.dtype == ATTN_F16 ? (d.D == 64 ? launch_tree_tc<H, 64> : launch_tree_tc<H, 128>)
                                       : (d.D == 64 ? launch_tree_tc<N, 64> : launch_tree_tc<N, 128>);
     return launch(d, p, dev, s);
   }
-  auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_mma<H, E, 128>
-                                           : d.D == 64 ? launch_tree_mma<H, H, 64> : launch_tree_mma<H, H, 128>)
-                                    : (fp8 ? launch_tree_mma<N, E, 128>
-                                           : d.D == 64 ? launch_tree_mma<N, N, 64> : launch_tree_mma<N, N, 128>);
-  return launch(d, p, dev, s);
+  auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_few<H, E, 128>
+                                           : d.D == 64 ? launch_tree_few<H, H, 64> : launch_tree_few<H, H, 128>)
+                                    : (fp8 ? launch_tree_few<N, E, 128>
+                                           : d.D == 64 ? launch_tree_few<N, N, 64> : launch_tree_few<N, N, 128>);
+  return launch(d, p, rows, dev, s);
 }
 
 template <typename Desc>
