@@ -254,6 +254,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   const int quad = lane & 3, grp = lane >> 2;
   const uint32_t s_q32 = attn_sm100::smem_u32(s_q);
   const float scale2 = p.scale * kLog2e;
+  // Where a lane reads in a group of 16 keys: e4m3 keys (row grp, chunk quad),
+  // e4m3 values (rows 2 quad and 2 quad + 1, chunk grp), and the addresses that
+  // it gives ldmatrix for 16-bit keys and values.
+  const uint32_t lane_k = grp * 128 + ((quad ^ grp) * 16);
+  const uint32_t lane_v0 = 2 * quad * 128 + ((grp ^ (2 * quad)) * 16);
+  const uint32_t lane_v1 = (2 * quad + 1) * 128 + ((grp ^ (2 * quad + 1)) * 16);
+  const uint32_t lane_k16 = ((lane & 7) + 8 * (lane >> 4)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) * 16);
+  const uint32_t lane_v16 = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
   int n = 0;
   bool ok = true;
   while (next_piece(p, split, share, pc)) {
@@ -354,13 +362,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int kb_end = cached ? 16 * C::kGroups * (warp + 1) : 16 * (warp + 1);
       for (int kb = cached ? 16 * C::kGroups * warp : 16 * warp; kb < min(kb_end, here) && ok; kb += 16 * NG) {
         float s[NG][MT][2][4];
-        uint32_t kbase[NG], vbase[NG];  // of the group's page segment
-        int r0[NG];                     // its first row there
+        // The group's first row in its page segment.  Groups start on multiples
+        // of 16 rows, so the swizzle of a row goes by the lane alone.
+        uint32_t kbase[NG], vbase[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const int j = kb + 16 * g, seg = j >> seg_shift;
-          r0[g] = j & ((1 << seg_shift) - 1);
-          const uint32_t off = seg * ((cached ? C::kRowBytes : C::kNewRowBytes) << seg_shift);
+          const uint32_t off = seg * ((cached ? C::kRowBytes : C::kNewRowBytes) << seg_shift) +
+                               (j & ((1 << seg_shift) - 1)) * 128;
           kbase[g] = ks + off, vbase[g] = vs + off;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
@@ -376,10 +385,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int r = r0[g] + 8 * h + grp;
-                w[g][h] = lds128(kbase[g] + r * 128 + (((quad + 4 * c) ^ (r & 7)) * 16));
-              }
+              for (int h = 0; h < 2; ++h)
+                w[g][h] = lds128(kbase[g] + h * 1024 + (lane_k ^ (64 * c)));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -400,12 +407,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         } else {
 #pragma unroll
           for (int x = 0; x < kSteps; ++x) {
-            const int chunk = 2 * x + ((lane >> 3) & 1);
 #pragma unroll
             for (int g = 0; g < (FP8 ? 1 : NG); ++g) {
-              const int r = r0[g] + (lane & 7) + 8 * (lane >> 4);
               uint32_t b[4];
-              ldmatrix4(b, kbase[g] + (chunk >> 3) * (128 << seg_shift) + r * 128 + (((chunk & 7) ^ (r & 7)) * 16));
+              ldmatrix4(b, kbase[g] + (x >> 2) * (128 << seg_shift) + (lane_k16 ^ (32 * (x & 3))));
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
                 uint32_t a[4];
@@ -484,10 +489,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
               top[mt][x] = fmaxf(top[mt][x], __shfl_xor_sync(0xffffffffu, top[mt][x], d));
+        // The running maxima move when one of a warp's rows grows by 2^4 past
+        // its own (weights stay below 2^(kShift + 4)): most tiles rescale nothing.
         bool moved = false;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) moved = moved || top[mt][0] != m[mt][0] || top[mt][1] != m[mt][1];
-        if (__any_sync(0xffffffffu, moved)) {
+        for (int mt = 0; mt < MT; ++mt) moved = moved || top[mt][0] > m[mt][0] + 4.f || top[mt][1] > m[mt][1] + 4.f;
+        if (!__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) top[mt][0] = m[mt][0], top[mt][1] = m[mt][1];
+        } else {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -549,8 +559,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
               uint32_t w[4][4];
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                const int r = r0[g] + 2 * quad + (y & 1) + 8 * (y >> 1);
-                const uint4 v = lds128(vbase[g] + r * 128 + ((grp ^ (r & 7)) * 16));
+                const uint4 v = lds128(vbase[g] + (y >> 1) * 1024 + (y & 1 ? lane_v1 : lane_v0));
                 w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
               }
               if (tail) {
@@ -578,9 +587,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
                 uint32_t w[4][4];
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                  const int r = r0[g] + 2 * quad + (y & 1) + 8 * (y >> 1), chunk = 2 * grp + c;
-                  const uint4 v = lds128(vbase[g] + (chunk >> 3) * (128 << seg_shift) + r * 128 +
-                                         (((chunk & 7) ^ (r & 7)) * 16));
+                  const int r = 2 * quad + (y & 1), chunk = 2 * grp + c;
+                  const uint4 v = lds128(vbase[g] + (chunk >> 3) * (128 << seg_shift) + (y >> 1) * 1024 + r * 128 +
+                                         (((chunk & 7) ^ r) * 16));
                   w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
                   if (j0 + (y & 1) + 8 * (y >> 1) >= here) w[y][0] = w[y][1] = w[y][2] = w[y][3] = 0u;
                 }
@@ -595,14 +604,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
               }
             }
           } else {
-            const int r = r0[g] + (lane & 7) + 8 * ((lane >> 3) & 1);
             const uint32_t live0 = (j0 < here ? 0xffffu : 0u) | (j0 + 1 < here ? 0xffff0000u : 0u);
             const uint32_t live1 = (j0 + 8 < here ? 0xffffu : 0u) | (j0 + 9 < here ? 0xffff0000u : 0u);
 #pragma unroll
             for (int t = 0; t < kTilesD / 2; ++t) {
-              const int chunk = 2 * t + (lane >> 4);
               uint32_t b[4];
-              ldmatrix4t(b, vbase[g] + (chunk >> 3) * (128 << seg_shift) + r * 128 + (((chunk & 7) ^ (r & 7)) * 16));
+              ldmatrix4t(b, vbase[g] + (t >> 2) * (128 << seg_shift) + (lane_v16 ^ (32 * (t & 3))));
               if (tail) b[0] &= live0, b[1] &= live1, b[2] &= live0, b[3] &= live1;
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {

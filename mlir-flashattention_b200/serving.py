@@ -19,18 +19,17 @@ run empty) is recorded in the runtime's status word, which ``check_status`` rais
 from __future__ import annotations
 
 import ctypes
-import struct
+import os
 from typing import NamedTuple
 
 import torch
 
-from . import ATTN_BF16, ATTN_E4M3, ATTN_F16, ATTN_F32, VerifyError, _raise, lib
+from . import _HERE, LIB_PATH, AttentionError, VerifyError, lib
 
 __all__ = ["AttnCachePlan", "AttnCacheAppend", "AttnRotary", "AttnTree", "CachePlan", "RotaryTable",
            "cache_plan", "cache_append", "rotary_table", "rotary", "fused_tree"]
 
 _I, _Q, _P, _F = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
-_DEVICE_POINTERS = 1  # flags: tensors here are known to be CUDA tensors
 
 
 class AttnCachePlan(ctypes.Structure):
@@ -65,44 +64,24 @@ class AttnTree(ctypes.Structure):
                 ("scale", _F), ("k_descale", _F), ("v_descale", _F), ("status", _P)]
 
 
-def _packer(cls):
-    """struct.Struct with the C layout of a descriptor: one pack() fills it in a microsecond, which
-    assigning forty ctypes fields does not."""
-    code = {_I: "i", _Q: "q", _P: "P", _F: "f", _Q * 2: "2q", _Q * 3: "3q"}
-    s = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_) + "0q")
-    assert s.size == ctypes.sizeof(cls)
-    return s.pack
+_module = None
 
 
-_pack_plan, _pack_append, _pack_rotary, _pack_tree = (
-    _packer(c) for c in (AttnCachePlan, AttnCacheAppend, AttnRotary, AttnTree))
-
-_CODES = {torch.float32: ATTN_F32, torch.bfloat16: ATTN_BF16, torch.float16: ATTN_F16,
-          torch.float8_e4m3fn: ATTN_E4M3, torch.uint8: ATTN_E4M3}
-
-_entries = {}
-
-
-def _entry(name):
-    fn = _entries.get(name)
-    if fn is None:
-        fn = getattr(lib(), name)
-        fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
-        _entries[name] = fn
-    return fn
-
-
-def _call(name, desc, device):
-    """Run an entry on the current stream of `device`."""
-    index = device.index
-    fn = _entry(name)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(desc, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(desc, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _raise(rc)
+def _native():
+    """The calls on torch tensors (_serving.so: checks, descriptors, the current stream)."""
+    global _module
+    if _module is None:
+        import importlib.util  # noqa: PLC0415
+        lib()
+        path = os.path.join(_HERE, "_serving.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"_serving.so not found at {path}; build it with __graft_entry__.build()")
+        spec = importlib.util.spec_from_file_location("_serving", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.setup(LIB_PATH, VerifyError, AttentionError)
+        _module = m
+    return _module
 
 
 def _on_stream(stream):
@@ -113,23 +92,6 @@ def _on_stream(stream):
 def _need(ok, message):
     if not ok:
         raise VerifyError(message)
-
-
-def _cuda(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise VerifyError(f"{name} must be a CUDA tensor on {device} (got {t.device})")
-
-
-def _ints(t, name, shape, dtype=torch.int32):
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-        raise VerifyError(f"{name} must be a contiguous {str(dtype)[6:]} tensor of shape {list(shape)} "
-                          f"(got {str(t.dtype)[6:]} {list(t.shape)})")
-
-
-def _no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise VerifyError(f"{what} has no backward pass: call it under torch.no_grad()")
 
 
 # ------------------------------------------------------------------ page planner
@@ -162,75 +124,11 @@ def cache_plan(lengths, targets, block_table, free_pages, free_count, page_size,
             return cache_plan(lengths, targets, block_table, free_pages, free_count, page_size, tokens,
                               lengths_out=lengths_out, free_count_out=free_count_out, slots=slots,
                               positions=positions, starts=starts)
-    _need(lengths.dim() == 1 and block_table.dim() == 2 and free_pages.dim() == 1,
-          "lengths must be [B], block_table [B, W] and free_pages [num_pages]")
-    B, W = block_table.shape
-    shape, device = lengths.shape, lengths.device
-    _need(device.type == "cuda", "lengths must be a CUDA tensor")
-    _need(shape[0] == B, "lengths and block_table must have one row per request")
-    _ints(lengths, "lengths", shape)
-    _ints(targets, "targets", shape)
-    _ints(free_pages, "free_pages", free_pages.shape)
-    _ints(free_count, "free_count", (1,))
-    _need(block_table.dtype == torch.int32 and (W <= 1 or block_table.stride(1) == 1),
-          "block_table must be int32 with unit-stride columns")
-    tokens = int(tokens)
-    _need(tokens >= 0, "tokens must not be negative")
-    if lengths_out is None:
-        lengths_out = torch.empty_like(lengths)
-    else:
-        _ints(lengths_out, "lengths_out", shape)
-    if free_count_out is None:
-        free_count_out = torch.empty_like(free_count)
-    else:
-        _ints(free_count_out, "free_count_out", (1,))
-    if slots is None:
-        slots = torch.empty(tokens, dtype=torch.int64, device=device)
-    else:
-        _ints(slots, "slots", (tokens,), torch.int64)
-    if positions is None:
-        positions = torch.empty(tokens, dtype=torch.int32, device=device)
-    else:
-        _ints(positions, "positions", (tokens,))
-    if starts is None:
-        starts = torch.empty(B + 1, dtype=torch.int32, device=device)
-    else:
-        _ints(starts, "starts", (B + 1,))
-    _cuda(device, targets=targets, block_table=block_table, free_pages=free_pages, free_count=free_count,
-          lengths_out=lengths_out, free_count_out=free_count_out, slots=slots, positions=positions, starts=starts)
-    desc = _pack_plan(_DEVICE_POINTERS, int(page_size), B, W, free_pages.shape[0], tokens,
-                      block_table.stride(0) if B > 1 else W, lengths.data_ptr(), targets.data_ptr(),
-                      block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), lengths_out.data_ptr(),
-                      free_count_out.data_ptr(), starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), 0)
-    _call("attn_cache_plan", desc, device)
-    return CachePlan(slots, positions, starts, lengths_out, free_count_out)
+    return CachePlan._make((_module or _native()).plan(lengths, targets, block_table, free_pages, free_count, page_size,
+                                                       tokens, lengths_out, free_count_out, slots, positions, starts))
 
 
 # ------------------------------------------------------------------ cache writer
-def _descale(value, name, heads, device):
-    """(factor, pointer) of a descale: a number, or one f32 value per key head."""
-    if isinstance(value, torch.Tensor):
-        if value.dtype != torch.float32 or value.shape != (heads,) or not value.is_contiguous() or value.device != device:
-            raise VerifyError(f"{name} must be a number or a contiguous f32 tensor of {heads} heads on {device}")
-        return 1.0, value.data_ptr()
-    return value, 0
-
-
-def _check_cache(k_cache, v_cache, heads, dim, code, device):
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != heads or k_cache.shape[3] != dim:
-        raise VerifyError(f"k_cache and v_cache must be [num_pages, {heads}, page_size, {dim}] "
-                          f"(got {list(k_cache.shape)} and {list(v_cache.shape)})")
-    if k_cache.dtype != v_cache.dtype or _CODES.get(k_cache.dtype, -1) not in (code, ATTN_E4M3):
-        raise VerifyError(f"k_cache and v_cache must share one type: that of the keys, or float8_e4m3fn "
-                          f"(got {k_cache.dtype} and {v_cache.dtype})")
-    if k_cache.device != device or v_cache.device != device:
-        raise VerifyError(f"k_cache and v_cache must be CUDA tensors on {device}")
-    ks, vs = k_cache.stride(), v_cache.stride()
-    if ks[3] != 1 or vs[3] != 1:
-        raise VerifyError("the cache's head_dim must be unit-stride")
-    return ks, vs
-
-
 def cache_append(k, v, k_cache, v_cache, slots, *, rows=None, k_descale=1.0, v_descale=1.0, stream=None):
     """Write rows of ``k`` and ``v`` [T, Hkv, D] (bf16 or f16) to their cache slots, in place.
 
@@ -241,31 +139,7 @@ def cache_append(k, v, k_cache, v_cache, slots, *, rows=None, k_descale=1.0, v_d
     if stream is not None:
         with _on_stream(stream):
             return cache_append(k, v, k_cache, v_cache, slots, rows=rows, k_descale=k_descale, v_descale=v_descale)
-    if k.dim() != 3 or k.shape != v.shape:
-        raise VerifyError("k and v must both be [tokens, heads, head_dim]")
-    T, H, D = k.shape
-    device, code = k.device, _CODES.get(k.dtype, -1)
-    if device.type != "cuda" or v.device != device:
-        raise VerifyError("k and v must be CUDA tensors on one device")
-    if v.dtype != k.dtype or code not in (ATTN_BF16, ATTN_F16):
-        raise VerifyError("k and v must both be bfloat16 or both float16")
-    a, b = k.stride(), v.stride()
-    if a[2] != 1 or b[2] != 1:
-        raise VerifyError("head_dim must be unit-stride")
-    ks, vs = _check_cache(k_cache, v_cache, H, D, code, device)
-    n = slots.shape[0] if slots.dim() else 0
-    _ints(slots, "slots", (n,), torch.int64)
-    if rows is not None:
-        _ints(rows, "rows", (n,))
-    _cuda(device, slots=slots, rows=rows)
-    _no_grad("cache_append", k, v)
-    kd, kp = _descale(k_descale, "k_descale", H, device)
-    vd, vp = _descale(v_descale, "v_descale", H, device)
-    desc = _pack_append(_DEVICE_POINTERS, code, _CODES[k_cache.dtype], k_cache.shape[2], n, T, H, D, k_cache.shape[0],
-                        a[0], a[1], b[0], b[1], *ks[:3], *vs[:3], k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
-                        v_cache.data_ptr(), slots.data_ptr(), rows.data_ptr() if rows is not None else 0, kp, vp, kd,
-                        vd, 0)
-    _call("attn_cache_append", desc, device)
+    (_module or _native()).append(k, v, k_cache, v_cache, slots, rows, k_descale, v_descale)
 
 
 # ------------------------------------------------------------------ rotary positions
@@ -293,77 +167,6 @@ def rotary_table(dim, sections=None, base=10000.0, *, interleaved=False, neighbo
     return RotaryTable(freqs.to(device), torch.tensor(axes, dtype=torch.int32, device=device), bool(neighbours))
 
 
-def _heads_strides(x, name, device, dtype):
-    """(B, H, N, D, strides of batch, head, token) of [T, H, D] or [B, H, N, D]."""
-    if x.device != device or x.dtype != dtype:
-        raise VerifyError(f"{name} must be a {str(dtype)[6:]} tensor on {device}")
-    s, n = x.stride(), x.shape
-    if len(n) == 4:
-        r = n[0], n[1], n[2], n[3], (s[0], s[1], s[2])
-    elif len(n) == 3:
-        r = 1, n[1], n[0], n[2], (0, s[1], s[0])
-    else:
-        raise VerifyError(f"{name} must be [tokens, heads, head_dim] or [batch, heads, tokens, head_dim]")
-    if s[-1] != 1:
-        raise VerifyError(f"{name} head_dim must be unit-stride")
-    return r
-
-
-def _rotate(q, k, positions, freqs, axes, neighbours, inverse, outs=(None, None)):
-    first = q if q is not None else k
-    device, dtype = first.device, first.dtype
-    code = _CODES.get(dtype, -1)
-    if device.type != "cuda":
-        raise VerifyError("Q and K must be CUDA tensors")
-    if code not in (ATTN_F32, ATTN_BF16, ATTN_F16):
-        raise VerifyError(f"rotary takes float32, bfloat16 or float16 (got {dtype})")
-    B, Hq, N, D, qs = _heads_strides(first, "Q", device, dtype)
-    Hk, ks, q_out, k_out = 0, (0, 0, 0), outs[0], outs[1]
-    if k is not None:
-        b2, Hk, n2, d2, ks = _heads_strides(k, "K", device, dtype)
-        if (b2, n2, d2) != (B, N, D) or k.dim() != first.dim():
-            raise VerifyError("Q and K must have the same tokens and head_dim")
-        if k_out is None:
-            k_out = torch.empty_like(k)
-    if q is None:
-        Hq, qs = 0, (0, 0, 0)
-    elif q_out is None:
-        q_out = torch.empty_like(q)
-    half = freqs.shape[0] if freqs.dim() else 0
-    if freqs.dtype != torch.float64 or freqs.shape != (half,) or not freqs.is_contiguous():
-        raise VerifyError("freqs must be a contiguous float64 tensor [dim / 2]")
-    if 2 * half > D:
-        raise VerifyError(f"freqs turn {2 * half} values of a head_dim of {D}")
-    if axes is not None:
-        _ints(axes, "axes", (half,))
-    p = positions
-    if p.dtype not in (torch.int32, torch.int64):
-        raise VerifyError("positions must be int32 or int64")
-    if p.dim() == 1:
-        p = p.unsqueeze(0)
-    ps = p.stride()
-    if p.dim() == 3 and first.dim() == 4 and p.shape[1:] == (B, N):
-        pos_stride = ps
-    elif p.dim() == 2 and p.shape[1] == N:
-        pos_stride = (ps[0], 0, ps[1])
-    else:
-        raise VerifyError(f"positions must be [axes, {N}]" + (f" or [axes, {B}, {N}]" if first.dim() == 4 else "") +
-                          f" (got {list(positions.shape)})")
-    if p.shape[0] == 0:
-        raise VerifyError("positions need an axis")
-    _cuda(device, positions=p, freqs=freqs, axes=axes)
-    zero = (0, 0, 0)
-    qos = _heads_strides(q_out, "q output", device, dtype)[4] if q is not None else zero
-    kos = _heads_strides(k_out, "k output", device, dtype)[4] if k is not None else zero
-    desc = _pack_rotary(_DEVICE_POINTERS, code, p.dtype == torch.int64, p.shape[0], bool(neighbours), bool(inverse), B, N,
-                        Hq, Hk, D, 2 * half, *qs, *ks, *qos, *kos, *pos_stride, q.data_ptr() if q is not None else 0,
-                        k.data_ptr() if k is not None else 0, q_out.data_ptr() if q is not None else 0,
-                        k_out.data_ptr() if k is not None else 0, p.data_ptr(), freqs.data_ptr(),
-                        axes.data_ptr() if axes is not None else 0, 0)
-    _call("attn_rotary", desc, device)
-    return q_out, k_out
-
-
 class _Rotary(torch.autograd.Function):
     """A turn; its gradient is the turn back, itself a turn (so differentiable again)."""
 
@@ -372,7 +175,7 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions, freqs, axes)
         ctx.how = neighbours, inverse
         ctx.set_materialize_grads(False)
-        return _rotate(q, k, positions, freqs, axes, neighbours, inverse)
+        return _native().rotate(q, k, positions, freqs, axes, neighbours, inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -385,9 +188,9 @@ class _Rotary(torch.autograd.Function):
 
 
 def _apply_rotary(q, k, positions, freqs, axes, neighbours, inverse):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+    if ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         return _Rotary.apply(q, k, positions, freqs, axes, neighbours, inverse)
-    return _rotate(q, k, positions, freqs, axes, neighbours, inverse)
+    return (_module or _native()).rotate(q, k, positions, freqs, axes, neighbours, inverse)
 
 
 def rotary(q, k, positions, freqs, axes=None, *, neighbours=False, inverse=False, stream=None):
@@ -403,8 +206,6 @@ def rotary(q, k, positions, freqs, axes=None, *, neighbours=False, inverse=False
     """
     if isinstance(freqs, RotaryTable):
         freqs, axes, neighbours = freqs
-    if q is None and k is None:
-        raise VerifyError("rotary needs Q or K")
     if stream is not None:
         with _on_stream(stream):
             return _apply_rotary(q, k, positions, freqs, axes, neighbours, inverse)
@@ -434,51 +235,5 @@ def fused_tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, 
         with _on_stream(stream):
             return fused_tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, scale, mask=mask,
                               max_new=max_new, output=output, lse=lse, k_descale=k_descale, v_descale=v_descale)
-    if q.dim() != 3 or k_new.dim() != 3 or k_new.shape != v_new.shape:
-        raise VerifyError("Q, K and V must be [tokens, heads, head_dim]")
-    T, Hq, D = q.shape
-    Tk, H, Dk = k_new.shape
-    if Tk != T:
-        raise VerifyError("K seq_len must equal Q seq_len")
-    if Dk != D:
-        raise VerifyError("K head_dim must equal Q head_dim")
-    device, code = q.device, _CODES.get(q.dtype, -1)
-    if device.type != "cuda" or k_new.device != device or v_new.device != device:
-        raise VerifyError("Q, K and V must be CUDA tensors on one device")
-    if code not in (ATTN_BF16, ATTN_F16) or k_new.dtype != q.dtype or v_new.dtype != q.dtype:
-        raise VerifyError("Q, K and V must share one element type, bfloat16 or float16")
-    qs, ns, ws = q.stride(), k_new.stride(), v_new.stride()
-    if qs[2] != 1 or ns[2] != 1 or ws[2] != 1:
-        raise VerifyError("head_dim must be unit-stride")
-    ks, vs = _check_cache(k_cache, v_cache, H, D, code, device)
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise VerifyError("block_table must be int32 [B, W] with unit-stride columns")
-    B, W = block_table.shape
-    _ints(lengths, "lengths", (B,))
-    _ints(starts, "starts", (B + 1,))
-    max_new = T if max_new is None else int(max_new)
-    mask_stride = 0
-    if mask is not None:
-        if (mask.dim() != 2 or mask.dtype not in (torch.bool, torch.uint8) or mask.shape[0] != T or
-                mask.shape[1] < max_new or (mask.shape[1] > 1 and mask.stride(1) != 1)):
-            raise VerifyError(f"mask must be bool [{T}, at least max_new = {max_new}] with unit-stride columns")
-        mask_stride = mask.stride(0) if T > 1 else mask.shape[1]
-    if output is None:
-        output = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-    elif output.shape != q.shape or output.dtype != q.dtype or output.stride(2) != 1:
-        raise VerifyError("output must have Q's shape and type, head_dim unit-stride")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, Hq) or not lse.is_contiguous()):
-        raise VerifyError("lse must be a contiguous f32 tensor [tokens, heads]")
-    _cuda(device, block_table=block_table, lengths=lengths, starts=starts, mask=mask, output=output, lse=lse)
-    _no_grad("fused_tree", q, k_new, v_new)
-    kd, kp = _descale(k_descale, "k_descale", H, device)
-    vd, vp = _descale(v_descale, "v_descale", H, device)
-    os = output.stride()
-    desc = _pack_tree(_DEVICE_POINTERS, code, _CODES[k_cache.dtype], k_cache.shape[2], B, T, Hq, H, D, W, k_cache.shape[0],
-                      max_new, qs[0], qs[1], ns[0], ns[1], ws[0], ws[1], os[0], os[1], *ks[:3], *vs[:3],
-                      block_table.stride(0) if B > 1 else W, mask_stride, q.data_ptr(), k_new.data_ptr(),
-                      v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), output.data_ptr(),
-                      lse.data_ptr() if lse is not None else 0, block_table.data_ptr(), lengths.data_ptr(),
-                      starts.data_ptr(), mask.data_ptr() if mask is not None else 0, kp, vp, scale, kd, vd, 0)
-    _call("attn_tree_fwd", desc, device)
-    return output
+    return (_module or _native()).tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, scale, mask, max_new,
+                                       output, lse, k_descale, v_descale)
