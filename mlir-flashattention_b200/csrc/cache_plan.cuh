@@ -25,6 +25,7 @@ namespace cache_plan {
 
 constexpr int kMaxRequests = 8192;
 constexpr int kMaxWarps = 32;
+constexpr int kRun = 4;  // tokens that a thread takes at once
 
 struct Params {
   int B, W, page_shift;
@@ -81,6 +82,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   int* const tok_pre = held + p.B;        // [B + 1]
   int* const grow_pre = tok_pre + p.B + 1;
   int* const drop_pre = grow_pre + p.B + 1;
+  int* const keeps = drop_pre + p.B + 1;  // [B] pages after the call
   __shared__ Sums warp_sums[kMaxWarps];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -105,6 +107,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
       }
       const int old_pages = (L + round_up) >> p.page_shift;
       const int new_pages = (G + round_up) >> p.page_shift;
+      keeps[b] = new_pages;
       v.tokens = max(0, G - L);
       v.grown = max(0, new_pages - old_pages);
       v.dropped = max(0, old_pages - new_pages);
@@ -112,18 +115,18 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
     const Sums inc = warp_scan(v, lane);
     if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
-    Sums before = run;
-    for (int w = 0; w < warps; ++w) {
-      const Sums s = warp_sums[w];
-      if (w < warp) {
-        before.tokens += s.tokens;
-        before.grown += s.grown;
-        before.dropped += s.dropped;
-      }
-      run.tokens += s.tokens;
-      run.grown += s.grown;
-      run.dropped += s.dropped;
+    if (warp == 0) {
+      const Sums s = warp_scan(lane < warps ? warp_sums[lane] : Sums{0, 0, 0}, lane);
+      if (lane < warps) warp_sums[lane] = s;
     }
+    __syncthreads();
+    Sums before = run;
+    if (warp > 0) {
+      const Sums s = warp_sums[warp - 1];
+      before.tokens += s.tokens, before.grown += s.grown, before.dropped += s.dropped;
+    }
+    const Sums all = warp_sums[warps - 1];
+    run.tokens += all.tokens, run.grown += all.grown, run.dropped += all.dropped;
     if (b < p.B) {
       // Saturated: a total past `tokens` refuses the whole call below.
       tok_pre[b] = static_cast<int>(min(before.tokens + inc.tokens - v.tokens, int64_t{0x7fffffff}));
@@ -154,8 +157,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   // Index x of the given-back pages: a table entry past its request's new end.
   auto given_back = [&](int x) {
     const int b = owner(drop_pre, p.B, x);
-    const int left = (p.targets[b] + round_up) >> p.page_shift;
-    return p.table[b * p.table_stride + left + (x - drop_pre[b])];
+    return p.table[b * p.table_stride + keeps[b] + (x - drop_pre[b])];
   };
   // k-th page taken from the stack.
   auto popped = [&](int k) {
@@ -163,19 +165,50 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
     return i < F ? p.free_pages[i] : given_back(i - F);
   };
 
-  for (int i = first; i < p.tokens; i += step) {
-    int64_t slot = -1;
-    int pos = 0;
-    if (i < total) {
-      const int b = owner(tok_pre, p.B, i);
-      const int L = held[b];
-      pos = L + (i - tok_pre[b]);
-      const int j = pos >> p.page_shift, have = (L + round_up) >> p.page_shift;
-      const int page = j < have ? p.table[b * p.table_stride + j] : popped(grow_pre[b] + j - have);
-      slot = (static_cast<int64_t>(page) << p.page_shift) + (pos & round_up);
+  // Runs of consecutive tokens: one search for the request, one page id for
+  // the tokens that share it, 16-byte stores.
+  const int per = p.tokens > step ? kRun : 1;
+  const bool aligned = per == kRun && (reinterpret_cast<uintptr_t>(p.slots) & 15u) == 0 &&
+                    (reinterpret_cast<uintptr_t>(p.positions) & 15u) == 0;
+  for (int i0 = first * per; i0 < p.tokens; i0 += step * per) {
+    int64_t slot[kRun];
+    int position[kRun];
+    int b = -1, page = 0, have = 0;
+    const int32_t* row = nullptr;
+#pragma unroll
+    for (int x = 0; x < kRun; ++x) {
+      const int i = i0 + x;
+      slot[x] = -1, position[x] = 0;
+      if (x >= per || i >= total) continue;
+      const bool next = b < 0 || i >= tok_pre[b + 1];
+      if (next) {
+        if (b < 0) b = owner(tok_pre, p.B, i);
+        else while (i >= tok_pre[b + 1]) ++b;
+        have = (held[b] + round_up) >> p.page_shift;
+        row = p.table + b * p.table_stride;
+      }
+      const int pos = held[b] + (i - tok_pre[b]);
+      if (next || (pos & round_up) == 0) {
+        const int j = pos >> p.page_shift;
+        page = j < have ? row[j] : popped(grow_pre[b] + j - have);
+      }
+      position[x] = pos;
+      slot[x] = (static_cast<int64_t>(page) << p.page_shift) + (pos & round_up);
     }
-    p.slots[i] = slot;
-    if (p.positions) p.positions[i] = pos;
+    if (aligned && i0 + kRun <= p.tokens) {
+#pragma unroll
+      for (int x = 0; x < kRun; x += 2)
+        *reinterpret_cast<longlong2*>(p.slots + i0 + x) = make_longlong2(slot[x], slot[x + 1]);
+      if (p.positions)
+        *reinterpret_cast<int4*>(p.positions + i0) = make_int4(position[0], position[1], position[2], position[3]);
+    } else {
+#pragma unroll
+      for (int x = 0; x < kRun; ++x) {
+        if (x >= per || i0 + x >= p.tokens) continue;
+        p.slots[i0 + x] = slot[x];
+        if (p.positions) p.positions[i0 + x] = position[x];
+      }
+    }
   }
   for (int b = first; b <= p.B; b += step) p.starts[b] = ok ? tok_pre[b] : 0;
   if (ok) {

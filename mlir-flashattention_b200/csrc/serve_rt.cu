@@ -63,6 +63,12 @@ bool stride_ok(int64_t stride, int64_t extent, int64_t multiple) {
   return extent <= 1 || stride % multiple == 0;
 }
 
+int pow2_shift(int64_t n, int lo, int hi) {
+  int s = lo;
+  while (s < hi && (int64_t{1} << s) < n) ++s;
+  return s;
+}
+
 constexpr int64_t kInt32 = (int64_t{1} << 31) - 1;
 
 // ------------------------------------------------------------------- plan
@@ -116,13 +122,13 @@ int run(const AttnCachePlan& d, cudaStream_t s) {
   p.positions = d.positions;
   p.slots = d.slots;
   p.status = d.status ? d.status : dev.status;
-  const size_t smem = (4 * static_cast<size_t>(d.B) + 3) * sizeof(int);
+  const size_t smem = (5 * static_cast<size_t>(d.B) + 3) * sizeof(int);
   static std::once_flag once[64];
   static cudaError_t attr[64];
   std::call_once(once[dev.index], [&] {
     attr[dev.index] = cudaFuncSetAttribute(cache_plan::plan_kernel,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (4 * cache_plan::kMaxRequests + 3) * int{sizeof(int)});
+                                           (5 * cache_plan::kMaxRequests + 3) * int{sizeof(int)});
   });
   if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "cudaFuncSetAttribute");
   const int64_t work = std::max(d.B, d.tokens);
@@ -209,14 +215,17 @@ int run(const AttnCacheAppend& d, cudaStream_t s) {
   p.k_descale_heads = d.k_descale_heads, p.v_descale_heads = d.v_descale_heads;
   p.k_descale = d.k_descale, p.v_descale = d.v_descale;
   p.status = d.status ? d.status : dev.status;
-  const int64_t units = d.N * p.Hkv * p.chunks * 2;
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, dev.sms * 64));
+  // Rows per block: two chunks a thread where there are rows enough to fill
+  // the GPU, else one row a block.
+  const int per_row = p.Hkv * p.chunks;
+  p.tile = d.N <= 4 * dev.sms ? 1 : std::max(1, 2 * cache_append::kThreads / per_row);
+  const unsigned blocks = static_cast<unsigned>((d.N + p.tile - 1) / p.tile);
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
   auto kern = d.dtype == ATTN_F16
                   ? (fp8 ? cache_append::append_kernel<true, true> : cache_append::append_kernel<true, false>)
                   : (fp8 ? cache_append::append_kernel<false, true>
                          : cache_append::append_kernel<false, false>);
-  kern<<<blocks, 256, 0, s>>>(p);
+  kern<<<blocks, cache_append::kThreads, 0, s>>>(p);
   return launched("cache_append launch");
 }
 
@@ -293,9 +302,17 @@ int run(const AttnRotary& d, cudaStream_t s) {
     if (o.heads > 0)
       wide = wide && aligned(o.ptr, 16) && stride_ok(o.st[0], d.B, vec) && stride_ok(o.st[1], o.heads, vec) &&
              stride_ok(o.st[2], d.N, vec);
-  // Tokens per block: about two packs a thread, and angles within 32 KB.
-  const int per_token = p.H * (p.D - p.half) / (wide ? vec : 1);
-  p.tile = std::max(1, 2 * rotary::kThreads / std::max(1, per_token));
+  // Units of a head: two packs each (one by one where rows are not aligned).
+  const int per_head = !wide ? p.D - p.half
+                             : ((2 * p.half / vec) + 1) / 2 + ((p.D - 2 * p.half) / vec + 1) / 2;
+  p.lanes_shift = pow2_shift(per_head, 0, 8);
+  p.heads_shift = p.H > 1 ? pow2_shift(p.H, 0, 8) - (p.H & (p.H - 1) ? 1 : 0) : 0;  // rounded down
+  // Tokens per block: eight units a thread where there are tokens enough to
+  // fill the GPU so, else one; and angles within 32 KB.
+  const int per_token = std::max(1, p.H << p.lanes_shift);
+  const int64_t units = p.tokens * per_token;
+  const int each = units >= int64_t{8} * rotary::kThreads * 8 * dev.sms ? 8 : 1;
+  p.tile = std::max(1, each * rotary::kThreads / per_token);
   if (p.half > 0) p.tile = std::max(1, std::min(p.tile, 4096 / p.half));
   switch (d.dtype) {
     case ATTN_F32: return wide ? launch_rotary<float, 4>(d, p, s) : launch_rotary<float, 1>(d, p, s);
@@ -464,12 +481,6 @@ cudaError_t prepare_kernels(K kern, J join, size_t smem, int threads, int pool) 
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, kern);
   if (e == cudaSuccess && fa.numRegs * threads < pool) e = cudaErrorLaunchOutOfResources;
   return e;
-}
-
-int pow2_shift(int64_t n, int lo, int hi) {
-  int s = lo;
-  while (s < hi && (int64_t{1} << s) < n) ++s;
-  return s;
 }
 
 template <typename T, typename TC, int D, int MT>
