@@ -12,7 +12,8 @@
 //   warps 4-7    softmax of accumulator 1
 //   warp 10      cuts the block's share into pieces, ahead of the others, and
 //                hands them out through a short queue in shared memory
-//   warp 11      idle (it completes warpgroup 2 for the register split)
+//   warp 11      with a mask, turns the mask's bytes into bits in shared memory
+//                ahead of the softmax (else idle)
 // In the tiles at the end of the cached and of the new keys the softmax also
 // makes the value rows that do not exist 0 in shared memory: their weights are
 // 0, but what lies in memory there need not be a number.
@@ -40,20 +41,22 @@ namespace tc {
 using namespace attn_sm100;
 
 constexpr int kThreads = 384;
-constexpr int kRegsSoftmax = 224, kRegsOther = 56;
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kRegPool = 256 * kRegsSoftmax + 128 * kRegsOther;
 constexpr int kTileRows = 128, kTileKeys = 128;
 
-template <typename T, int D>
+template <typename T, int D, bool MASK>
 struct Cfg {
   static constexpr bool F16 = std::is_same<T, __half>::value;
   static constexpr int kHalves = D / 64;               // 128-byte column blocks
   static constexpr int kBox = kTileKeys * 128;         // one column block of a tile
   static constexpr int kTile = kHalves * kBox;
-  static constexpr int kStages = D == 128 ? 5 : 12;    // K and V tiles in the ring
+  // K and V tiles in the ring; mask bits take the room of one.
+  static constexpr int kStages = (D == 128 ? 5 : 12) - (MASK ? 1 : 0);
+  static constexpr int kBits = MASK ? 256 : 0;         // 16-byte rows of mask bits, twice
   static constexpr int kQueue = 4;                     // pieces handed out ahead
-  static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 3 + 2 * kQueue;
-  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + kBars * 8 + 16 + kQueue * 64;
+  static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 3 + 2 * kQueue + 4;
+  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + 2 * kBits * 16 + kBars * 8 + 16 + kQueue * 64;
   static constexpr float kShift = F16 ? 8.f : 0.f;     // weights are kept times 2^kShift
   static constexpr float kLazy = F16 ? 6.f : 8.f;      // below 2^(kShift + kLazy): 2^14 in f16
   static_assert(kSmem + 512 <= 232448, "shared memory budget");
@@ -153,29 +156,20 @@ __device__ __forceinline__ void mask_row(const uint8_t* row, int here, uint32_t 
   }
 }
 
-// Not inlined: it runs once or twice an item, and its loads would take the
-// registers of every tile's softmax.
-__device__ __noinline__ uint4 mask_row_bits(const uint8_t* row, int here, int align) {
-  uint32_t b[4];
-  if (align >= 16) mask_row<16>(row, here, b);
-  else if (align >= 4) mask_row<4>(row, here, b);
-  else mask_row<1>(row, here, b);
-  return make_uint4(b[0], b[1], b[2], b[3]);
-}
-
-template <typename T, int D>
+template <typename T, int D, bool MASK>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kc,
                    const __grid_constant__ CUtensorMap map_vc, const __grid_constant__ CUtensorMap map_kn,
                    const __grid_constant__ CUtensorMap map_vn, const __grid_constant__ Params p, const Split split,
                    const Tiles tiles, const Scratch scratch, const int min_units) {
-  using C = Cfg<T, D>;
+  using C = Cfg<T, D, MASK>;
   constexpr bool F16 = C::F16;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   uint8_t* const sQ = smem;
   uint8_t* const sKV = smem + 2 * C::kTile;
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(sKV + C::kStages * C::kTile);
+  uint4* const s_bits = reinterpret_cast<uint4*>(sKV + C::kStages * C::kTile);  // [2][tokens of an item]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_bits + 2 * C::kBits);
   uint64_t* const q_full = bars;
   uint64_t* const q_empty = bars + 1;
   uint64_t* const kv_full = bars + 2;
@@ -188,7 +182,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* const drain = met + 1;
   uint64_t* const job_full = drain + 1;
   uint64_t* const job_empty = job_full + C::kQueue;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(job_empty + C::kQueue);
+  uint64_t* const bits_full = job_empty + C::kQueue;
+  uint64_t* const bits_empty = bits_full + 2;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bits_empty + 2);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Job* const jobs = reinterpret_cast<Job*>(tmem_slot + 4);
 
@@ -211,7 +207,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(drain, 1);
     for (int i = 0; i < C::kQueue; ++i) {
       mbar_init(&job_full[i], 1);
-      mbar_init(&job_empty[i], 10);  // producer, issuer and eight softmax warps
+      mbar_init(&job_empty[i], MASK ? 11 : 10);  // producer, issuer, eight softmax warps, warp 11
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bits_full[i], 1);
+      mbar_init(&bits_empty[i], 8);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -432,6 +432,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!more) break;
       }
       __syncwarp();
+    } else if constexpr (MASK) {
+      // ---------------------------------------------------- mask bits (warp 11)
+      int turn = 0;  // new tiles so far
+      bool ok = true;
+      Job j;
+      for (int n = 0; ok && take_job(n, j); ++n) {
+        leave_job(n);
+        const int tokens = (j.rows + p.group - 1) / p.group;
+        const int64_t row0 = j.first + j.rt * split.rows / p.group;
+        for (int k = max(j.k0, j.cached); k < j.k1 && ok; ++k, ++turn) {
+          const int buf = turn & 1, here = j.here(split, k);
+          ok = wait(&bits_empty[buf], static_cast<uint32_t>((turn >> 1) & 1) ^ 1u);
+          if (!ok) break;
+          for (int i = lane; i < tokens; i += 32) {
+            const uint8_t* const row = p.mask + (row0 + i) * p.mask_stride + ((k - j.cached) << split.new_shift);
+            uint32_t b[4];
+            if (p.mask_align >= 16) mask_row<16>(row, here, b);
+            else if (p.mask_align >= 4) mask_row<4>(row, here, b);
+            else mask_row<1>(row, here, b);
+            s_bits[buf * C::kBits + i] = make_uint4(b[0], b[1], b[2], b[3]);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bits_full[buf]);
+        }
+      }
+      __syncwarp();
     }
   } else {
     setmaxnreg_inc<kRegsSoftmax>();
@@ -447,28 +473,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     int steps = 0;  // S tiles of this accumulator so far
     int base = 0;   // ring position of the piece's first K
     int meets = 0;  // phases of `met` so far
+    int turns = 0;  // new tiles of the pieces before
     bool ok = true;
-    Job j;
-    for (int n = 0; ok && take_job(n, j); ++n) {
-      leave_job(n);
-      const int row0 = j.alone ? 0 : t * tiles.rows;  // of the item
+    for (int n = 0; ok; ++n) {
+      ok = wait(&job_full[n % C::kQueue], static_cast<uint32_t>((n / C::kQueue) & 1));
+      if (!ok) break;
+      // Read in place: only what every tile needs stays in registers.
+      const Job& j = jobs[n % C::kQueue];
+      if (j.b < 0) break;
+      const int k0 = j.k0, cached_end = j.cached, held = j.held, count = j.count;
+      const bool alone = j.alone;
+      const int row0 = alone ? 0 : t * tiles.rows;  // of the item
       const int rows = min(tiles.rows, j.rows - row0);
       const int at = j.rt * split.rows + row0 + min(r, max(rows, 1) - 1);
       const int token = at / p.group;
       const bool busy = (warp & 3) * 32 < rows;  // a warp without rows only keeps step
       float m = -INFINITY, l = 0.f;
       const int from = j.from(t), stop = j.stop(t);
-      for (int k = from; k < stop && ok; k += j.step(), ++steps) {
-        const bool cached = k < j.cached;
-        const int here = j.here(split, k);
-        uint32_t bits[4];
-        const bool masked = !cached && p.mask != nullptr && busy;
-        if (masked) {
-          const uint8_t* const row = p.mask + static_cast<int64_t>(j.first + token) * p.mask_stride +
-                                     ((k - j.cached) << split.new_shift);
-          const uint4 b = mask_row_bits(row, here, p.mask_align);
-          bits[0] = b.x, bits[1] = b.y, bits[2] = b.z, bits[3] = b.w;
-        }
+      for (int k = from; k < stop && ok; k += alone ? 2 : 1, ++steps) {
+        const bool cached = k < cached_end;
+        const int here = cached ? min(kTileKeys, held - (k << split.keys_shift))
+                                : min(1 << split.new_shift, count - ((k - cached_end) << split.new_shift));
         ok = wait(&s_full[t], static_cast<uint32_t>(steps & 1));
         if (!ok) break;
         tc_fence_after();
@@ -476,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // Accumulator 0's products of a tile come first.  The tile before in
           // V's slot has been used (S of this one is complete), so the phase
           // waited for is the slot's next.
-          const int vp = base + 2 * (k - j.k0) + 1;
+          const int vp = base + 2 * (k - k0) + 1;
           ok = wait(&kv_full[slot(vp)], par(vp));
           if (!ok) break;
           if (r >= here) {
@@ -487,6 +512,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(v + c * C::kBox + x * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
+        }
+        int buf = 0;
+        if constexpr (MASK) {
+          if (!cached) {
+            // The turn of this tile among the block's new tiles.
+            const int turn = turns + k - max(k0, cached_end);
+            buf = turn & 1;
+            ok = wait(&bits_full[buf], static_cast<uint32_t>((turn >> 1) & 1));
+            if (!ok) break;
+          }
         }
         float s[128];
         if (busy) {
@@ -504,12 +539,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             s[96 + i] = __uint_as_float(r3[i]);
           }
           int lim = here;  // keys below it are seen
-          if (masked) {
+          if (!cached && !MASK) lim = min(here, token - ((k - cached_end) << split.new_shift) + 1);
+          if constexpr (MASK) {
+            if (!cached) {
+              const uint4 b = s_bits[buf * C::kBits + (row0 + min(r, max(rows, 1) - 1)) / p.group];
+              const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if ((bits[c >> 5] >> (c & 31)) & 1u) s[c] = hidden;
-          } else if (!cached) {
-            lim = min(here, token - ((k - j.cached) << split.new_shift) + 1);
+              for (int c = 0; c < 128; ++c)
+                if ((bits[c >> 5] >> (c & 31)) & 1u) s[c] = hidden;
+            }
           }
           if (__any_sync(0xffffffffu, lim < 128)) {
 #pragma unroll
@@ -554,6 +592,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           l *= alpha;
         }
+        if constexpr (MASK) {
+          if (!cached) {  // alone: the other group does not read this tile's bits
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&bits_empty[buf]);
+              if (alone) mbar_arrive(&bits_empty[buf]);
+            }
+          }
+        }
         // Weights in two halves, each published as it is stored.
         const float sub = m == -INFINITY ? 0.f : C::kShift - m;
         const uint64_t sl2x2 = f2_pack(sl2, sl2), subx2 = f2_pack(sub, sub);
@@ -585,6 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       base += 2 * (j.k1 - j.k0);
+      turns += max(0, j.k1 - max(j.k0, j.cached));
       // ------------------------------------------------------------ a piece ends
       const bool has = from < stop, whole = j.whole;
       if (has && !wait(&pv_done[t], static_cast<uint32_t>((steps - 1) & 1))) break;
@@ -661,6 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               none ? -INFINITY : (mm - C::kShift + log2f(ll)) * kLn2;
         }
       }
+      leave_job(n);
     }
   }
   tc_fence_before();
@@ -678,7 +727,7 @@ constexpr int kJoinThreads = 512, kJoinRows = 32;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     tree_tc_join(const __grid_constant__ Params p, const Scratch scratch) {
-  using C = Cfg<T, D>;
+  using C = Cfg<T, D, false>;
   constexpr int kCols = D / 4 / (kJoinThreads / 32);
   grid_wait();
   grid_release();

@@ -534,10 +534,10 @@ int launch_tree_few(const AttnTree& d, const attn_tree::Params& p, int64_t rows,
   return launch_tree_mma<T, TC, D, 2>(d, p, dev, s);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool MASK>
 int launch_tree_tc(const AttnTree& d, const attn_tree::Params& p, const rt_host::Device& dev, cudaStream_t s) {
-  using C = attn_tree::tc::Cfg<T, D>;
-  auto kern = attn_tree::tc::tree_tc_kernel<T, D>;
+  using C = attn_tree::tc::Cfg<T, D, MASK>;
+  auto kern = attn_tree::tc::tree_tc_kernel<T, D, MASK>;
   static std::once_flag once[64];
   static cudaError_t attr[64];
   std::call_once(once[dev.index], [&] {
@@ -622,8 +622,13 @@ int run(const AttnTree& d, cudaStream_t s) {
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
   const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
   if (!fp8 && rows > (d.D == 64 ? 64 : 32)) {
-    auto launch = d.dtype == ATTN_F16 ? (d.D == 64 ? launch_tree_tc<H, 64> : launch_tree_tc<H, 128>)
-                                      : (d.D == 64 ? launch_tree_tc<N, 64> : launch_tree_tc<N, 128>);
+    if (d.mask) {
+      auto launch = d.dtype == ATTN_F16 ? (d.D == 64 ? launch_tree_tc<H, 64, true> : launch_tree_tc<H, 128, true>)
+                                        : (d.D == 64 ? launch_tree_tc<N, 64, true> : launch_tree_tc<N, 128, true>);
+      return launch(d, p, dev, s);
+    }
+    auto launch = d.dtype == ATTN_F16 ? (d.D == 64 ? launch_tree_tc<H, 64, false> : launch_tree_tc<H, 128, false>)
+                                      : (d.D == 64 ? launch_tree_tc<N, 64, false> : launch_tree_tc<N, 128, false>);
     return launch(d, p, dev, s);
   }
   auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_few<H, E, 128>
