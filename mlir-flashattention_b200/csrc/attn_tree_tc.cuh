@@ -45,18 +45,20 @@ constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kRegPool = 256 * kRegsSoftmax + 128 * kRegsOther;
 constexpr int kTileRows = 128, kTileKeys = 128;
 
-template <typename T, int D, bool MASK>
+template <typename T, int D, bool MASK, bool ALONE>
 struct Cfg {
   static constexpr bool F16 = std::is_same<T, __half>::value;
   static constexpr int kHalves = D / 64;               // 128-byte column blocks
   static constexpr int kBox = kTileKeys * 128;         // one column block of a tile
   static constexpr int kTile = kHalves * kBox;
-  // K and V tiles in the ring; mask bits take the room of one.
-  static constexpr int kStages = (D == 128 ? 5 : 12) - (MASK ? 1 : 0);
+  // K and V tiles in the ring.  Mask bits take the room of one; a second Q tile
+  // that no item has leaves one.
+  static constexpr int kQTiles = ALONE ? 1 : 2;
+  static constexpr int kStages = (D == 128 ? 7 : 14) - kQTiles - (MASK ? 1 : 0);
   static constexpr int kBits = MASK ? 256 : 0;         // 16-byte rows of mask bits, twice
   static constexpr int kQueue = 4;                     // pieces handed out ahead
   static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 3 + 2 * kQueue + 4;
-  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + 2 * kBits * 16 + kBars * 8 + 16 + kQueue * 64;
+  static constexpr size_t kSmem = 1024 + (kQTiles + kStages) * kTile + 2 * kBits * 16 + kBars * 8 + 16 + kQueue * 64;
   static constexpr float kShift = F16 ? 8.f : 0.f;     // weights are kept times 2^kShift
   static constexpr float kLazy = F16 ? 6.f : 8.f;      // below 2^(kShift + kLazy): 2^14 in f16
   static_assert(kSmem + 512 <= 232448, "shared memory budget");
@@ -91,6 +93,19 @@ struct Job {
   __device__ __forceinline__ int from(int t) const { return alone ? k0 + t : k0; }
   __device__ __forceinline__ int step() const { return alone ? 2 : 1; }
   __device__ __forceinline__ int stop(int t) const { return min(t ? end1 : end0, k1); }
+  // Places in the ring, from the piece's first on: K, V of each tile in turn, or
+  // (early: ALONE, where two tiles are in work) K_0, K_1, V_0, K_2, V_1, .., the
+  // order of use, so that no slot is held for a V that is two products away.
+  template <bool EARLY>
+  __device__ __forceinline__ int k_place(int k) const {
+    const int i = k - k0;
+    return EARLY ? max(2 * i - 1, 0) : 2 * i;
+  }
+  template <bool EARLY>
+  __device__ __forceinline__ int v_place(int k) const {
+    const int i = k - k0;
+    return EARLY && k + 1 < k1 ? 2 * i + 2 : 2 * i + 1;
+  }
   // Keys that exist in tile k.
   __device__ __forceinline__ int here(const Split& s, int k) const {
     return k < cached ? min(kTileKeys, held - (k << s.keys_shift))
@@ -156,18 +171,19 @@ __device__ __forceinline__ void mask_row(const uint8_t* row, int here, uint32_t 
   }
 }
 
-template <typename T, int D, bool MASK>
+// ALONE: no request has more rows than one tile, so that every item is alone.
+template <typename T, int D, bool MASK, bool ALONE>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kc,
                    const __grid_constant__ CUtensorMap map_vc, const __grid_constant__ CUtensorMap map_kn,
                    const __grid_constant__ CUtensorMap map_vn, const __grid_constant__ Params p, const Split split,
                    const Tiles tiles, const Scratch scratch, const int min_units) {
-  using C = Cfg<T, D, MASK>;
+  using C = Cfg<T, D, MASK, ALONE>;
   constexpr bool F16 = C::F16;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   uint8_t* const sQ = smem;
-  uint8_t* const sKV = smem + 2 * C::kTile;
+  uint8_t* const sKV = smem + C::kQTiles * C::kTile;
   uint4* const s_bits = reinterpret_cast<uint4*>(sKV + C::kStages * C::kTile);  // [2][tokens of an item]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(s_bits + 2 * C::kBits);
   uint64_t* const q_full = bars;
@@ -262,23 +278,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (k >= min(j.cached, j.k1) || lane >= segments(k)) return 0;
           return __ldg(row + (((k << split.keys_shift) + (lane << seg_shift)) >> p.page_shift));
         };
-        int page_next = page_of(j.k0);
-        for (int k = j.k0; k < j.k1 && ok; ++k) {
-          const bool cached = k < j.cached;
-          const int segs = cached ? segments(k) : 1;
-          int page = page_next, at = 0;
-          page_next = page_of(k + 1);  // a tile ahead of its use
-          if (cached && lane < segs) {
-            at = ((k << split.keys_shift) + (lane << seg_shift)) & ((1 << p.page_shift) - 1);
-            if (page < 0 || page >= p.num_pages) {
-              atomicCAS(p.status, 0, ATTN_ERR_INVALID);
-              page = max(p.num_pages, 1);  // outside the map: zeros
+        // K and V of a tile share its page ids, which are read a tile ahead.
+        constexpr int kLag = ALONE ? 1 : 0;
+        int page_next = page_of(j.k0), page_last = 0;
+        for (int k = j.k0; k < j.k1 + kLag && ok; ++k) {
+          const int page_here = page_next;
+          page_next = page_of(k + 1);
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const int kk = v ? k - kLag : k;
+            if (kk < j.k0 || kk >= j.k1) continue;
+            const bool cached = kk < j.cached;
+            const int segs = cached ? segments(kk) : 1;
+            int page = v && ALONE ? page_last : page_here, at = 0;
+            if (cached && lane < segs) {
+              at = ((kk << split.keys_shift) + (lane << seg_shift)) & ((1 << p.page_shift) - 1);
+              if (page < 0 || page >= p.num_pages) {
+                atomicCAS(p.status, 0, ATTN_ERR_INVALID);
+                page = max(p.num_pages, 1);  // outside the map: zeros
+              }
             }
-          }
-          for (int v = 0; v < 2; ++v, ++pos) {
             const int s = slot(pos);
             ok = wait(&kv_empty[s], par(pos) ^ 1u);
             if (!ok) break;
+            ++pos;
             const int seg = 128 << (cached ? seg_shift : split.new_shift);
             if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], segs * seg * C::kHalves);
             __syncwarp();
@@ -290,17 +313,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                   tma_load_5d(dst + c * C::kBox, v ? &map_vc : &map_kc, &kv_full[s], 0, at, c, j.h, page);
                 else
                   tma_load_5d(dst + c * C::kBox, v ? &map_vn : &map_kn, &kv_full[s], 0,
-                              j.first + ((k - j.cached) << split.new_shift), c, j.h, 0);
+                              j.first + ((kk - j.cached) << split.new_shift), c, j.h, 0);
               }
             }
           }
+          page_last = page_here;
           if (k == j.k0 && ok) {
             // Q behind the piece's first keys, which need not wait for the
             // last S product of the piece before.
             ok = wait(q_empty, static_cast<uint32_t>(n & 1) ^ 1u);
             if (!ok) break;
             if (lane == 0) {
-              const int m = j.alone ? 1 : 2;
+              const int m = ALONE || j.alone ? 1 : 2;
               mbar_arrive_expect_tx(q_full, m * C::kHalves * tiles.rows * 128);
               for (int t = 0; t < m; ++t)
                 for (int c = 0; c < C::kHalves; ++c)
@@ -335,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Job j;
       for (; ok && take_job(n, j); ++n) {
         leave_job(n);
-        auto kpos = [&](int k) { return base + 2 * (k - j.k0); };
+        auto kpos = [&](int k) { return base + j.template k_place<ALONE>(k); };
         int left = 0;  // S products still to issue from this Q
         for (int t = 0; t < 2; ++t) {
           const int f = j.from(t), e = j.stop(t);
@@ -370,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j.from(t) < j.stop(t)) ok = issue_S(t, j.from(t));
         bool first_pv[2] = {true, true}, waited = n == 0;
         for (int k = j.k0; k < j.k1 && ok; ++k) {
-          const int vp = kpos(k) + 1;
+          const int vp = base + j.template v_place<ALONE>(k);
           ok = wait(&kv_full[slot(vp)], par(vp));
           for (int t = 0; t < 2 && ok; ++t) {
             if (!j.takes(t, k)) continue;
@@ -501,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // Accumulator 0's products of a tile come first.  The tile before in
           // V's slot has been used (S of this one is complete), so the phase
           // waited for is the slot's next.
-          const int vp = base + 2 * (k - k0) + 1;
+          const int vp = base + j.template v_place<ALONE>(k);
           ok = wait(&kv_full[slot(vp)], par(vp));
           if (!ok) break;
           if (r >= here) {
@@ -538,21 +562,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             s[64 + i] = __uint_as_float(r2[i]);
             s[96 + i] = __uint_as_float(r3[i]);
           }
-          int lim = here;  // keys below it are seen
-          if (!cached && !MASK) lim = min(here, token - ((k - cached_end) << split.new_shift) + 1);
+          // Bits of the keys that this row does not see.
+          uint32_t hide[4] = {0, 0, 0, 0};
+          const int lim = cached || MASK ? here : min(here, token - ((k - cached_end) << split.new_shift) + 1);
+          if (lim < kTileKeys) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) hide[w] = lim >= 32 * w + 32 ? 0u : 0xffffffffu << max(lim - 32 * w, 0);
+          }
           if constexpr (MASK) {
             if (!cached) {
               const uint4 b = s_bits[buf * C::kBits + (row0 + min(r, max(rows, 1) - 1)) / p.group];
-              const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-              for (int c = 0; c < 128; ++c)
-                if ((bits[c >> 5] >> (c & 31)) & 1u) s[c] = hidden;
+              hide[0] |= b.x, hide[1] |= b.y, hide[2] |= b.z, hide[3] |= b.w;
             }
           }
-          if (__any_sync(0xffffffffu, lim < 128)) {
+          if (__any_sync(0xffffffffu, (hide[0] | hide[1] | hide[2] | hide[3]) != 0)) {
 #pragma unroll
             for (int c = 0; c < 128; ++c)
-              if (c >= lim) s[c] = hidden;
+              if ((hide[c >> 5] >> (c & 31)) & 1u) s[c] = hidden;
           }
           float red;
           if (pos) {
@@ -727,7 +753,7 @@ constexpr int kJoinThreads = 512, kJoinRows = 32;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
     tree_tc_join(const __grid_constant__ Params p, const Scratch scratch) {
-  using C = Cfg<T, D, false>;
+  using C = Cfg<T, D, false, false>;
   constexpr int kCols = D / 4 / (kJoinThreads / 32);
   grid_wait();
   grid_release();

@@ -534,10 +534,10 @@ int launch_tree_few(const AttnTree& d, const attn_tree::Params& p, int64_t rows,
   return launch_tree_mma<T, TC, D, 2>(d, p, dev, s);
 }
 
-template <typename T, int D, bool MASK>
+template <typename T, int D, bool MASK, bool ALONE>
 int launch_tree_tc(const AttnTree& d, const attn_tree::Params& p, const rt_host::Device& dev, cudaStream_t s) {
-  using C = attn_tree::tc::Cfg<T, D, MASK>;
-  auto kern = attn_tree::tc::tree_tc_kernel<T, D, MASK>;
+  using C = attn_tree::tc::Cfg<T, D, MASK, ALONE>;
+  auto kern = attn_tree::tc::tree_tc_kernel<T, D, MASK, ALONE>;
   static std::once_flag once[64];
   static cudaError_t attr[64];
   std::call_once(once[dev.index], [&] {
@@ -577,6 +577,15 @@ int launch_tree_tc(const AttnTree& d, const attn_tree::Params& p, const rt_host:
   if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
   rt_host::count_launches(2);
   return ATTN_OK;
+}
+
+// The kernel for many rows; a request of one row tile is alone with its keys.
+template <typename T, int D>
+int launch_tree_many(const AttnTree& d, const attn_tree::Params& p, int64_t rows, const rt_host::Device& dev,
+                     cudaStream_t s) {
+  if (rows <= attn_tree::tc::kTileRows / p.group * p.group)
+    return d.mask ? launch_tree_tc<T, D, true, true>(d, p, dev, s) : launch_tree_tc<T, D, false, true>(d, p, dev, s);
+  return d.mask ? launch_tree_tc<T, D, true, false>(d, p, dev, s) : launch_tree_tc<T, D, false, false>(d, p, dev, s);
 }
 
 int run(const AttnTree& d, cudaStream_t s) {
@@ -622,14 +631,9 @@ int run(const AttnTree& d, cudaStream_t s) {
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
   const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
   if (!fp8 && rows > (d.D == 64 ? 64 : 32)) {
-    if (d.mask) {
-      auto launch = d.dtype == ATTN_F16 ? (d.D == 64 ? launch_tree_tc<H, 64, true> : launch_tree_tc<H, 128, true>)
-                                        : (d.D == 64 ? launch_tree_tc<N, 64, true> : launch_tree_tc<N, 128, true>);
-      return launch(d, p, dev, s);
-    }
-    auto launch = d.dtype == ATTN_F16 ? (d.D == 64 ? launch_tree_tc<H, 64, false> : launch_tree_tc<H, 128, false>)
-                                      : (d.D == 64 ? launch_tree_tc<N, 64, false> : launch_tree_tc<N, 128, false>);
-    return launch(d, p, dev, s);
+    if (d.dtype == ATTN_F16)
+      return d.D == 64 ? launch_tree_many<H, 64>(d, p, rows, dev, s) : launch_tree_many<H, 128>(d, p, rows, dev, s);
+    return d.D == 64 ? launch_tree_many<N, 64>(d, p, rows, dev, s) : launch_tree_many<N, 128>(d, p, rows, dev, s);
   }
   auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_few<H, E, 128>
                                            : d.D == 64 ? launch_tree_few<H, H, 64> : launch_tree_few<H, H, 128>)
