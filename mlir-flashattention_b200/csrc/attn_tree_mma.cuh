@@ -11,10 +11,10 @@
 // A block is two teams and fills an SM; its registers are divided so that the
 // reading warps have 224 (setmaxnreg).  Tensor cores by mma.sync m16n8k16: operands go from
 // shared memory to registers, so 16 rows cost 16 rows (a 128-row accumulator
-// in tensor memory would be 1/8 used and its softmax one warp's work).  MT
-// 16-row tiles share every key that is read: 1 (decode), 2, or 4 at D = 64,
-// where mma.sync's own rate (a quarter of tcgen05's) still keeps up with the
-// memory; beyond, attn_tree_tc.cuh.
+// in tensor memory would be 1/8 used and its softmax one warp's work).  MT = 1
+// or 2 16-row tiles share every key that is read; from the third on the warps'
+// own instructions bound it (48 rows at D = 64: 125 us with four tiles, 111 us
+// in attn_tree_tc.cuh; 32 rows: 63 us here, 107 us there).
 //
 // An e4m3 cache is met in f16: e4m3 values are f16 values, and a bf16 row of q
 // scaled by the power of two that brings its largest value to 2^14..2^15 is

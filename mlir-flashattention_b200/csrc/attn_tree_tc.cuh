@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = wait(&s_full[t], static_cast<uint32_t>(steps & 1));
         if (!ok) break;
         tc_fence_after();
-        if (here < kTileKeys && (t == 0 || !j.takes(0, k))) {
+        if (__builtin_expect(here < kTileKeys, 0) && (t == 0 || !j.takes(0, k))) {
           // Accumulator 0's products of a tile come first.  The tile before in
           // V's slot has been used (S of this one is complete), so the phase
           // waited for is the slot's next.
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               hide[0] |= b.x, hide[1] |= b.y, hide[2] |= b.z, hide[3] |= b.w;
             }
           }
-          if (__any_sync(0xffffffffu, (hide[0] | hide[1] | hide[2] | hide[3]) != 0)) {
+          if (__builtin_expect(__any_sync(0xffffffffu, (hide[0] | hide[1] | hide[2] | hide[3]) != 0), 0)) {
 #pragma unroll
             for (int c = 0; c < 128; ++c)
               if ((hide[c >> 5] >> (c & 31)) & 1u) s[c] = hidden;
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             alpha = ex2(m - top);
             m = top;
           }
-          if (__any_sync(0xffffffffu, k != from && alpha != 1.f)) {
+          if (__builtin_expect(__any_sync(0xffffffffu, k != from && alpha != 1.f), 0)) {
             // The P V product before this S product is complete (see issue_S).
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {

@@ -522,15 +522,11 @@ int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, const rt_host
   return ATTN_OK;
 }
 
-// The kernel for few rows, with as many 16-row tiles as the rows of a request
-// need, up to 2 (at D = 64: 4).
+// The kernel for few rows, with one 16-row tile or two.
 template <typename T, typename TC, int D>
 int launch_tree_few(const AttnTree& d, const attn_tree::Params& p, int64_t rows, const rt_host::Device& dev,
                     cudaStream_t s) {
   if (rows <= 16) return launch_tree_mma<T, TC, D, 1>(d, p, dev, s);
-  if constexpr (D == 64) {
-    if (rows > 32) return launch_tree_mma<T, TC, D, 4>(d, p, dev, s);
-  }
   return launch_tree_mma<T, TC, D, 2>(d, p, dev, s);
 }
 
@@ -630,7 +626,7 @@ int run(const AttnTree& d, cudaStream_t s) {
   using E = __nv_fp8_e4m3;
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
   const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
-  if (!fp8 && rows > (d.D == 64 ? 64 : 32)) {
+  if (!fp8 && rows > 32) {
     if (d.dtype == ATTN_F16)
       return d.D == 64 ? launch_tree_many<H, 64>(d, p, rows, dev, s) : launch_tree_many<H, 128>(d, p, rows, dev, s);
     return d.D == 64 ? launch_tree_many<N, 64>(d, p, rows, dev, s) : launch_tree_many<N, 128>(d, p, rows, dev, s);
