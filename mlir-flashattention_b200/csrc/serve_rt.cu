@@ -584,6 +584,63 @@ int launch_tree_many(const AttnTree& d, const attn_tree::Params& p, int64_t rows
   return d.mask ? launch_tree_tc<T, D, true, false>(d, p, dev, s) : launch_tree_tc<T, D, false, false>(d, p, dev, s);
 }
 
+// The choice of kernel.
+int launch_tree(const AttnTree& d, const attn_tree::Params& p, const rt_host::Device& dev, cudaStream_t s) {
+  using H = __half;
+  using N = __nv_bfloat16;
+  using E = __nv_fp8_e4m3;
+  const bool fp8 = d.cache_dtype == ATTN_E4M3;
+  const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
+  if (!fp8 && rows > 32) {
+    if (d.dtype == ATTN_F16)
+      return d.D == 64 ? launch_tree_many<H, 64>(d, p, rows, dev, s) : launch_tree_many<H, 128>(d, p, rows, dev, s);
+    return d.D == 64 ? launch_tree_many<N, 64>(d, p, rows, dev, s) : launch_tree_many<N, 128>(d, p, rows, dev, s);
+  }
+  auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_few<H, E, 128>
+                                           : d.D == 64 ? launch_tree_few<H, H, 64> : launch_tree_few<H, H, 128>)
+                                    : (fp8 ? launch_tree_few<N, E, 128>
+                                           : d.D == 64 ? launch_tree_few<N, N, 64> : launch_tree_few<N, N, 128>);
+  return launch(d, p, rows, dev, s);
+}
+
+// With rows that may be hidden from a new key: values that are no numbers stay
+// where they are seen (see clean_values).
+template <typename T, int D>
+int launch_tree_hidden(const AttnTree& d, const attn_tree::Params& p, const rt_host::Device& dev, cudaStream_t s) {
+  constexpr int kThreads = attn_tree::kValueThreads;
+  auto clean = attn_tree::clean_values<T, D>;
+  auto whole = attn_tree::whole_values<T, D>;
+  static std::once_flag once[64];
+  static cudaError_t attr[64];
+  std::call_once(once[dev.index], [&] {
+    cudaError_t& e = attr[dev.index];
+    e = cudaFuncSetAttribute(clean, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(whole, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  });
+  if (attr[dev.index] != cudaSuccess) return cuda_fail(attr[dev.index], "set-up of a kernel");
+  const int64_t packs = d.T * d.Hkv * (D / 8);
+  const int blocks = static_cast<int>(std::min<int64_t>((packs + kThreads - 1) / kThreads, 4ll * dev.sms));
+  const size_t flags = round256(blocks * sizeof(int));
+  void* base = nullptr;
+  cudaError_t e = rt_host::scratch(&base, flags + packs * 16, s);
+  if (e != cudaSuccess) return cuda_fail(e, "stream-ordered scratch (new values)");
+  int* const odd = static_cast<int*>(base);
+  AttnTree c = d;
+  c.v_new = static_cast<char*>(base) + flags;
+  c.v_stride[0] = d.Hkv * D, c.v_stride[1] = D;
+  e = launch_early(clean, dim3(blocks), kThreads, 0, s, p, reinterpret_cast<uint4*>(static_cast<char*>(base) + flags),
+                   odd);
+  const int rc = e == cudaSuccess ? launch_tree(c, p, dev, s) : ATTN_OK;
+  if (e == cudaSuccess && rc == ATTN_OK)
+    e = launch_early(whole, dim3((d.Hkv * D + kThreads - 1) / kThreads), kThreads, 0, s, p, odd, blocks);
+  cudaFreeAsync(base, s);
+  if (rc != ATTN_OK) return rc;
+  if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");
+  rt_host::count_launches(2);
+  return ATTN_OK;
+}
+
 int run(const AttnTree& d, cudaStream_t s) {
   if (d.B == 0 || d.T == 0 || d.Hq == 0 || d.max_new == 0) return ATTN_OK;
   rt_host::Device dev;
@@ -621,21 +678,11 @@ int run(const AttnTree& d, cudaStream_t s) {
   p.k_descale_heads = d.k_descale_heads, p.v_descale_heads = d.v_descale_heads;
   p.scale = d.scale, p.k_descale = d.k_descale, p.v_descale = d.v_descale;
   p.status = d.status ? d.status : dev.status;
-  using H = __half;
-  using N = __nv_bfloat16;
-  using E = __nv_fp8_e4m3;
-  const bool fp8 = d.cache_dtype == ATTN_E4M3;
-  const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
-  if (!fp8 && rows > 32) {
-    if (d.dtype == ATTN_F16)
-      return d.D == 64 ? launch_tree_many<H, 64>(d, p, rows, dev, s) : launch_tree_many<H, 128>(d, p, rows, dev, s);
-    return d.D == 64 ? launch_tree_many<N, 64>(d, p, rows, dev, s) : launch_tree_many<N, 128>(d, p, rows, dev, s);
-  }
-  auto launch = d.dtype == ATTN_F16 ? (fp8 ? launch_tree_few<H, E, 128>
-                                           : d.D == 64 ? launch_tree_few<H, H, 64> : launch_tree_few<H, H, 128>)
-                                    : (fp8 ? launch_tree_few<N, E, 128>
-                                           : d.D == 64 ? launch_tree_few<N, N, 64> : launch_tree_few<N, N, 128>);
-  return launch(d, p, rows, dev, s);
+  if (p.max_new == 1 && !d.mask) return launch_tree(d, p, dev, s);
+  if (d.dtype == ATTN_F16)
+    return d.D == 64 ? launch_tree_hidden<__half, 64>(d, p, dev, s) : launch_tree_hidden<__half, 128>(d, p, dev, s);
+  return d.D == 64 ? launch_tree_hidden<__nv_bfloat16, 64>(d, p, dev, s)
+                   : launch_tree_hidden<__nv_bfloat16, 128>(d, p, dev, s);
 }
 
 template <typename Desc>

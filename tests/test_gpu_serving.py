@@ -518,6 +518,33 @@ def test_infinite_and_nan_keys_under_the_mask(pkg):
             assert bool(((t.o.cpu().double()[:8] - o).abs() <= tol)[keep].all())
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("Hq,H,new,held", [(4, 2, 8, 40), (16, 2, 8, 300), (32, 2, 8, 40), (32, 1, 40, 3000), (4, 4, 8, 9000)])
+def test_values_under_the_mask(pkg, dtype, cache, Hq, H, new, held):
+    """A drafted token's value that is infinite or no number reaches the rows that see it and no others, in items that
+    one block takes whole and in items cut between blocks."""
+    for mask in ("tree", None):
+        t = Tree(dtype, cache, Hq, H, 128, 16, [held, 3], [new, 2], mask, seed=24)
+        n = t.rows
+        t.v[5, 0, 3], t.v[5, 0, 70], t.v[5, H - 1, 127] = float("inf"), float("nan"), -float("inf")
+        t.run(pkg)
+        pkg.check_status(0)
+        clean = t.v[:n].nan_to_num(0, 0, 0)
+        o, _, a = ref.tree(t.q[:n], t.k[:n], clean, t.kc, t.vc, t.table, t.held, t.starts, t.scale, t.mask, t.kd, t.vd)
+        got = t.o.cpu().double()[:n]
+        for i in range(new):
+            if (t.mask is None and i >= 5) or (t.mask is not None and not t.mask[i, 5]):
+                for x in range(Hq // H):
+                    o[i, x, 3] = float("inf")
+                    o[i, x, 70] = float("nan")
+                    o[i, (H - 1) * (Hq // H) + x, 127] = -float("inf")
+        odd = ~o.isfinite()
+        assert torch.equal(got.isnan(), o.isnan()) and torch.equal(got[odd & ~o.isnan()], o[odd & ~o.isnan()])
+        u = half_step(dtype)
+        tol = u * o.abs() + 1.1 * u * a + 1e-6 * a.amax(-1, keepdim=True)
+        assert bool(((got - o).abs() <= tol)[~odd].all())
+
+
 def test_layouts(pkg):
     """Q, K, V from one fused projection, tokens outside heads in the cache, a padded table and mask."""
     t = Tree(BF16, BF16, 6, 2, 128, 32, [100, 33, 260], [3, 1, 9], "tree", seed=15)
