@@ -7,17 +7,17 @@
 // accumulator in 32 bits.
 //
 // This header: what the kernels share - operands, the requests as the device
-// arrays give them, and the split of the work.  attn_tree_mma.cuh holds the
-// kernel for few query rows and the join of split items.
+// arrays give them, the split of the work, and values that are no numbers.
+// attn_tree_mma.cuh holds the kernel for few query rows and the join of its
+// split items, attn_tree_tc.cuh those for many rows.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-
-#include <type_traits>
 #include <cuda_fp8.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/attn_rt.h"
 
