@@ -591,7 +591,11 @@ int launch_tree(const AttnTree& d, const attn_tree::Params& p, const rt_host::De
   using E = __nv_fp8_e4m3;
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
   const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
-  if (!fp8 && rows > 32) {
+  // Measured, us, by the mma kernel (row tiles of 32) and by tcgen05.  D = 64,
+  // 100 requests with a mask, 1500 keys: 40 rows 69 and 86, 48 rows 135 and
+  // 164, 64 rows 93 and 87, 96 rows 227 and 165.  D = 128: 40 rows 100 and 102,
+  // without a mask 98 and 86, 64 rows 132 and 87.
+  if (!fp8 && rows > (d.D == 64 ? 48 : 32)) {
     if (d.dtype == ATTN_F16)
       return d.D == 64 ? launch_tree_many<H, 64>(d, p, rows, dev, s) : launch_tree_many<H, 128>(d, p, rows, dev, s);
     return d.D == 64 ? launch_tree_many<N, 64>(d, p, rows, dev, s) : launch_tree_many<N, 128>(d, p, rows, dev, s);
