@@ -297,8 +297,9 @@ ATTN_API int attn_fwd_host_noalloc(const AttnDesc* desc, void* stream);
  * tables and slots are device data that the host never sees: what is wrong with
  * them is recorded in the status word (`status`, or the runtime's per-device
  * word when null; attn_rt_check_status) and the rows concerned are skipped.
- * Calls may be captured into CUDA graphs and run on several streams at once,
- * as long as the buffers they write differ. */
+ * Calls may be captured into CUDA graphs (after a first call of the kind on the
+ * device outside of a capture) and run on several streams at once, as long as
+ * the buffers they write differ. */
 #define ATTN_FLAG_DEVICE_POINTERS 1 /* flags: the caller vouches that every data
                                        pointer is device memory (not looked up)  */
 

@@ -348,8 +348,8 @@ __global__ void __launch_bounds__(kValueThreads)
   constexpr int kPacks = D / 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t rows = min(max(__ldg(p.starts + p.B), 0), p.T);
-  const int64_t n = rows * p.Hkv * kPacks;
+  const int64_t live = __ldg(p.starts + p.B);  // rows behind them may hold anything
+  const int64_t n = static_cast<int64_t>(p.T) * p.Hkv * kPacks;
   uint32_t met = 0;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kValueThreads) + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * kValueThreads) {
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kValueThreads)
     for (int k = 0; k < 4; ++k) {
       const uint32_t m = __vcmpeq2(x[k] & kExponent, kExponent);
       x[k] &= ~m;
-      met |= m;
+      if (row / p.Hkv < live) met |= m;
     }
     out[i] = w;
   }

@@ -230,6 +230,7 @@ def fused_tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, 
     itself and those before it: a decoded token, or a chunk of a prompt.  ``max_new`` bounds the new
     tokens of a request (default T).  A row that sees nothing gets O = 0 and LSE = -inf; rows past
     ``starts[B]`` are left as they were.  ``lse`` (f32 [T, Hq]) receives the natural-log sums.
+    ``output`` may be q itself, but must not overlap the other operands.
     """
     if stream is not None:
         with _on_stream(stream):

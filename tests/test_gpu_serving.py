@@ -565,6 +565,26 @@ def test_layouts(pkg):
     assert bool((out[:, :2] == 7).all()) and bool((out[:, 8:] == 7).all())
 
 
+@pytest.mark.parametrize("Hq,H,new,held", [(8, 2, 1, 9000), (16, 2, 5, 100), (32, 1, 40, 3000), (64, 8, 30, 50)])
+def test_output_over_q(pkg, Hq, H, new, held):
+    """The result may take q's place, whole items and cut ones, with the same bits."""
+    t = Tree(BF16, BF16, Hq, H, 128, 16, [held, 3, 70], [new, 1, new], "tree" if new > 1 else None, tail=0, seed=25).run(pkg)
+    q = t.q.cuda()
+    pkg.fused_tree(q, t.k.cuda(), t.v.cuda(), t.kc.cuda(), t.vc.cuda(), t.table.cuda(), ints(t.held),
+                   ints(t.starts), t.scale, mask=None if t.mask is None else t.mask.cuda(), max_new=t.max_new, output=q)
+    assert torch.equal(q.view(torch.int16), t.o.view(torch.int16))
+    t.check(pkg)
+
+
+def test_after_a_refused_plan_nothing_is_written(pkg):
+    """starts of 0, as a refused plan leaves them: no row belongs to a request."""
+    t = Tree(BF16, BF16, 8, 2, 128, 16, [40, 3], [3, 2], None, seed=26)
+    t.starts = [0, 0, 0]
+    t.run(pkg)
+    pkg.check_status(0)
+    assert bool((t.o == 7).all()) and bool((t.lse == 7).all())
+
+
 def test_descales_per_head(pkg):
     t = Tree(BF16, E4M3, 8, 4, 128, 16, [200, 10], [1, 7], seed=16)
     t.kd, t.vd = torch.tensor([0.5, 1.0, 0.1, 2.0]), torch.tensor([3.0, 0.2, 1.0, 0.6])
