@@ -12,11 +12,11 @@
 // reading warps have 224 (setmaxnreg).  Tensor cores by mma.sync m16n8k16:
 // operands go from shared memory to registers, so 16 rows cost 16 rows (a
 // 128-row accumulator in tensor memory would be 1/8 used and its softmax one
-// warp's work).  MT = 1 or 2 16-row tiles share every key that is read; more
-// than 32 rows are more than one item.  (Three tiles at D = 64, 48 rows on 8000
-// keys: 281 us against 351 in items of 32, but at 40 rows 157 against 152, and
-// slower in smaller calls.)  64 requests with 8192 keys, 8 kv-heads, bf16: 196
-// us, 6.1 TB/s.
+// warp's work).  MT = 1, 2 or (D = 64) 3 16-row tiles share every key that is
+// read; more rows are more items.  From there on the warps' own instructions
+// bound it (64 rows at D = 64 and 8000 keys: 219 us, 212 us in attn_tree_tc.cuh;
+// 128 rows 378 and 214).  64 requests with 8192 keys, 8 kv-heads, bf16: 196 us,
+// 6.1 TB/s.
 //
 // An e4m3 cache is met in f16: e4m3 values are f16 values, and a bf16 row of q
 // scaled by the power of two that brings its largest value to 2^14..2^15 is

@@ -522,11 +522,18 @@ int launch_tree_mma(const AttnTree& d, const attn_tree::Params& p, const rt_host
   return ATTN_OK;
 }
 
-// The kernel for few rows, with one 16-row tile or two.
+// The kernel for few rows, with one 16-row tile, two or (D = 64, more than 40
+// rows, work for every SM) three, which read each key once where two tiles are
+// two items.  Measured, us, 48 rows by three and by two: 256 items of up to 4096
+// keys 100 and 115, 800 of 8000 keys 281 and 351, of 100 keys 52 and 49; 32 items
+// 42 and 38.  40 rows: 400 items of 8000 keys 157 and 152, of 1500 81 and 69.
 template <typename T, typename TC, int D>
 int launch_tree_few(const AttnTree& d, const attn_tree::Params& p, int64_t rows, const rt_host::Device& dev,
                     cudaStream_t s) {
   if (rows <= 16) return launch_tree_mma<T, TC, D, 1>(d, p, dev, s);
+  if constexpr (D == 64) {
+    if (rows > 40 && d.B * d.Hkv >= dev.sms) return launch_tree_mma<T, TC, D, 3>(d, p, dev, s);
+  }
   return launch_tree_mma<T, TC, D, 2>(d, p, dev, s);
 }
 
@@ -591,7 +598,7 @@ int launch_tree(const AttnTree& d, const attn_tree::Params& p, const rt_host::De
   using E = __nv_fp8_e4m3;
   const bool fp8 = d.cache_dtype == ATTN_E4M3;
   const int64_t rows = static_cast<int64_t>(p.max_new) * p.group;
-  // Measured, us, by the mma kernel (row tiles of 32) and by tcgen05.  D = 64,
+  // Measured, us, by the mma kernel (two row tiles) and by tcgen05.  D = 64,
   // 100 requests with a mask, 1500 keys: 40 rows 69 and 86, 48 rows 135 and
   // 164, 64 rows 93 and 87, 96 rows 227 and 165.  D = 128: 40 rows 100 and 102,
   // without a mask 98 and 86, 64 rows 132 and 87.

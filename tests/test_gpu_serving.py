@@ -472,6 +472,18 @@ def test_blocks_take_several_tiles_and_items(pkg, dtype, cache, Hq, H, new):
          "tree" if new > 1 else None, seed=new).run(pkg).check(pkg)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("Hq,H,new,B", [(16, 4, 12, 40), (4, 4, 44, 37), (4, 4, 48, 3), (5, 1, 9, 150), (16, 4, 10, 40)])
+def test_rows_between_the_kernels(pkg, dtype, Hq, H, new, B):
+    """33 to 48 rows at D = 64, with items for every SM and with few."""
+    rng = random.Random(new)
+    held = [rng.randrange(0, 200) for _ in range(B)]
+    news = [rng.randrange(0, new + 1) for _ in range(B - 1)] + [new]
+    Tree(dtype, dtype, Hq, H, 64, 16, held, news, "tree", seed=27).run(pkg).check(pkg)
+    Tree(dtype, dtype, Hq, H, 64, 32, held, news, None, seed=28).run(pkg).check(pkg)
+    Tree(dtype, dtype, Hq, H, 64, 32, [9000] + held[1:], news, "empty", seed=29).run(pkg).check(pkg)
+
+
 def test_long_chunks(pkg):
     """Chains of many row tiles: more items than blocks, accumulators whose keys end at different tiles."""
     Tree(BF16, BF16, 16, 4, 128, 128, [300, 0], [1300, 900], seed=22).run(pkg).check(pkg)
