@@ -404,8 +404,9 @@ ATTN_API int attn_rotary(const AttnRotary* desc, void* stream);
  * token for decode, a chunk of a prompt).  With a mask, a drafted tree: mask
  * out all but a node's ancestors and itself.
  *   O = softmax(scale * q . k) . v over the visible keys,  LSE = ln of the sum
- * A row that sees nothing gives O = 0 and LSE = -inf.  Rows of q past
- * starts[B] are left as they were.  Keys and values of an e4m3 cache stand for
+ * A row that sees nothing gives O = 0 and LSE = -inf; one whose scores are no
+ * numbers gives O and LSE that are none, one whose scores are all -inf O = 0 / 0
+ * and LSE = -inf.  Rows of q past starts[B] are left as they were.  Keys and values of an e4m3 cache stand for
  * themselves times the descales; k_new and v_new have q's type. */
 typedef struct AttnTree {
   int32_t flags;

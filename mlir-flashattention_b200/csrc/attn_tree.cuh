@@ -301,6 +301,7 @@ struct alignas(32) Record {
   int row;     // first query row of the item in the request
   int rows;
   int h;
+  int held, count;  // of the request
 };
 
 struct Scratch {
@@ -322,8 +323,28 @@ __device__ __forceinline__ Record make_record(const Params& p, const Split& s, c
   r.rows = static_cast<int>(min(static_cast<int64_t>(s.rows), static_cast<int64_t>(pc.r.count) * p.group -
                                                                   static_cast<int64_t>(pc.rt) * s.rows));
   r.h = pc.h;
+  r.held = pc.r.held;
+  r.count = pc.r.count;
   return r;
 }
+
+// What a row's sum of values is divided by, as a factor.  The sum of weights is
+// 0 where every score was -inf: 0 for a row that sees no key, else 0 / 0.  (A
+// sum that is not a number passes through, and the maximum with it stays -inf
+// if all scores were none: pieces are joined relative to base_of.)
+__device__ __forceinline__ float over(const Params& p, float sum, int held, int first, int count, int token) {
+  if (sum != 0.f) return 1.f / sum;
+  bool sees = held > 0 || p.mask == nullptr;
+  if (!sees) {
+    const uint8_t* const row = p.mask + static_cast<int64_t>(first + token) * p.mask_stride;
+#pragma unroll 1
+    for (int j = 0; j < count && !sees; ++j) sees = row[j] == 0;
+  }
+  return sees ? __int_as_float(0x7fc00000) : 0.f;
+}
+
+// What weights are taken relative to: a maximum of -inf stands for no key yet.
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 
 template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }

@@ -661,12 +661,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kMmaWarps; ++w) top = fmaxf(top, warp_m[w][wr]);
-      if (top != -INFINITY) {
+      // A warp that met only scores that are no numbers has the maximum -inf and
+      // a sum that is none: it must not be lost.
 #pragma unroll
-        for (int w = 0; w < kMmaWarps; ++w) sum += attn_sm100::ex2(warp_m[w][wr] - top) * warp_l[w][wr];
-      }
+      for (int w = 0; w < kMmaWarps; ++w) sum += attn_sm100::ex2(warp_m[w][wr] - base_of(top)) * warp_l[w][wr];
       const int at = row0 + wr;
       const int token = pc.r.first + at / p.group, head = pc.h * p.group + at % p.group;
+      const float inv =
+          whole && writes ? over(p, sum, pc.r.held, pc.r.first, pc.r.count, at / p.group) : 0.f;
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += C::kJoinCols) {
         float* const mine = s_join + (warp * 16 + grp) * C::kJoinCols;  // + 8 rows
@@ -701,7 +703,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
             x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
           }
           if (whole) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
             *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + c0 + wc) =
                 make_uint2(pack2<F16>(x.x * inv, x.y * inv), pack2<F16>(x.z * inv, x.w * inv));
           } else {
@@ -771,16 +772,14 @@ __global__ void __launch_bounds__(kJoinThreads)
           }
         }
         const float high = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
-        if (high != -INFINITY) {
-          const float f = attn_sm100::ex2(top - high);
-          top = high;
-          sum *= f, a.x *= f, a.y *= f, a.z *= f, a.w *= f;
+        const float base = base_of(high), f = attn_sm100::ex2(top - base);
+        top = high;
+        sum *= f, a.x *= f, a.y *= f, a.z *= f, a.w *= f;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float w = attn_sm100::ex2(m[x] - high);
-            sum += w * l[x];
-            a.x += w * y[x].x, a.y += w * y[x].y, a.z += w * y[x].z, a.w += w * y[x].w;
-          }
+        for (int x = 0; x < 4; ++x) {
+          const float w = attn_sm100::ex2(m[x] - base);
+          sum += w * l[x];
+          a.x += w * y[x].x, a.y += w * y[x].y, a.z += w * y[x].z, a.w += w * y[x].w;
         }
       }
     }
@@ -790,9 +789,8 @@ __global__ void __launch_bounds__(kJoinThreads)
       if (g == 0) {
         for (int i = 1; i < G; ++i) {
           const int o = tid + i * kCols;
-          const float m = part_m[o], high = fmaxf(m, top);
-          if (high == -INFINITY) continue;
-          const float f = attn_sm100::ex2(top - high), w = attn_sm100::ex2(m - high);
+          const float m = part_m[o], high = fmaxf(m, top), base = base_of(high);
+          const float f = attn_sm100::ex2(top - base), w = attn_sm100::ex2(m - base);
           const float4 y = part_o[o];
           top = high;
           sum = sum * f + w * part_l[o];
@@ -802,8 +800,8 @@ __global__ void __launch_bounds__(kJoinThreads)
       __syncthreads();
     }
     if (g == 0 && row < row_hi) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int at = rec.row + row;
+      const float inv = over(p, sum, rec.held, rec.first, rec.count, at / p.group);
       const int token = rec.first + at / p.group, head = rec.h * p.group + at % p.group;
       *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + 4 * col) =
           make_uint2(pack2<F16>(a.x * inv, a.y * inv), pack2<F16>(a.z * inv, a.w * inv));

@@ -690,9 +690,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait(met, static_cast<uint32_t>(meets++ & 1))) break;
       }
       const bool live = r < rows;
-      const bool none = ll == 0.f;  // nothing seen: 0 whatever the accumulator holds
-      const float inv = whole && !none ? 1.f / ll : 1.f;
-      const float w0 = f0 * inv, w1 = f1 * inv;
+      const bool none = ll == 0.f;  // no weight: 0 or 0 / 0 whatever the accumulator holds
+      const float inv = whole && live ? over(p, ll, j.held, j.first, j.count, token) : 1.f;
+      const float w0 = f0 * inv, w1 = f1 * inv, nothing = whole && none ? inv : 0.f;
       const int head = j.h * p.group + at % p.group;
       T* const orow = static_cast<T*>(p.o) + static_cast<int64_t>(j.first + token) * p.o_st + head * p.o_sh;
       float4* const srow = scratch.o + static_cast<int64_t>(j.rec) * (D / 4) * 256 + row0 + r;
@@ -705,7 +705,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(tA + c, a);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) a[i] = any && !none ? __float_as_uint(__uint_as_float(a[i]) * w0) : 0u;
+          for (int i = 0; i < 32; ++i)
+            a[i] = any && !none ? __float_as_uint(__uint_as_float(a[i]) * w0) : __float_as_uint(nothing);
           if (two) {
             uint32_t b[32];
             tmem_ld32(tA + D + c, b);
@@ -787,24 +788,22 @@ __global__ void __launch_bounds__(kJoinThreads)
       }
     }
     const float high = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
-    if (high != -INFINITY) {
-      const float f = ex2(top - high);
-      top = high;
-      sum *= f;
+    const float base = base_of(high), f = ex2(top - base);
+    top = high;
+    sum *= f;
 #pragma unroll
-      for (int k = 0; k < kCols; ++k) a[k].x *= f, a[k].y *= f, a[k].z *= f, a[k].w *= f;
+    for (int k = 0; k < kCols; ++k) a[k].x *= f, a[k].y *= f, a[k].z *= f, a[k].w *= f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float w = ex2(m[x] - high);
-        sum += w * l[x];
+    for (int x = 0; x < 4; ++x) {
+      const float w = ex2(m[x] - base);
+      sum += w * l[x];
 #pragma unroll
-        for (int k = 0; k < kCols; ++k)
-          a[k].x += w * y[x][k].x, a[k].y += w * y[x][k].y, a[k].z += w * y[x][k].z, a[k].w += w * y[x][k].w;
-      }
+      for (int k = 0; k < kCols; ++k)
+        a[k].x += w * y[x][k].x, a[k].y += w * y[x][k].y, a[k].z += w * y[x][k].z, a[k].w += w * y[x][k].w;
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int at = rec.row + row;
+  const float inv = over(p, sum, rec.held, rec.first, rec.count, at / p.group);
   const int token = rec.first + at / p.group, head = rec.h * p.group + at % p.group;
   T* const out = static_cast<T*>(p.o) + token * p.o_st + head * p.o_sh + 4 * col;
 #pragma unroll
