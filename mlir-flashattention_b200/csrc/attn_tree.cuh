@@ -390,31 +390,70 @@ __global__ void __launch_bounds__(kValueThreads)
   if (threadIdx.x == 0) odd[blockIdx.x] = any;
 }
 
-// A thread has one column of one K/V head, so that no two change the same result.
+// A block takes rows_each rows of one request and K/V head, a thread a column and
+// every lanes-th row, so that no two change the same result.  What a row adds
+// goes by which of +inf, -inf and NaN it sees: without a mask by where each
+// comes first in the column, with one by a walk along the row's keys that ends
+// when nothing that comes can change it.  2 requests of 2048 tokens, 8 K/V
+// heads of 128, whose values are all NaN: 0.3 ms beside the attention's 0.2, under
+// a mask 0.4 beside 0.5.
 template <typename T, int D>
 __global__ void __launch_bounds__(kValueThreads)
-    whole_values(const __grid_constant__ Params p, const int* __restrict__ odd, const int flags) {
+    whole_values(const __grid_constant__ Params p, const int* odd, const int flags, const int rows_each,
+                 const int splits) {
+  constexpr int kLanes = kValueThreads / D, kNever = 0x7fffffff;
+  __shared__ int first[3][D];  // of +inf, -inf, NaN: the first row of the column
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int met = 0;
   for (int i = threadIdx.x; i < flags; i += kValueThreads) met |= odd[i];
   if (!__syncthreads_or(met)) return;
-  for (int b = 0; b < p.B; ++b) {
-    const Request r = request(p, b);
-    for (int c = blockIdx.x * kValueThreads + threadIdx.x; c < p.Hkv * D; c += gridDim.x * kValueThreads) {
-      const int h = c / D, col = c % D;
-      const T* const v = static_cast<const T*>(p.v_new) + r.first * p.v_st + h * p.v_sh + col;
+  const int col = threadIdx.x % D, lane = threadIdx.x / D;
+  const int64_t items = static_cast<int64_t>(p.B) * p.Hkv * splits;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int64_t bh = it / splits;
+    const int h = static_cast<int>(bh % p.Hkv);
+    const Request r = request(p, static_cast<int>(bh / p.Hkv));
+    const int lo = static_cast<int>(it % splits) * rows_each, hi = min(r.count, lo + rows_each);
+    if (lo >= hi) continue;  // for the whole block
+    const int end = p.mask ? r.count : hi;  // keys that these rows may see
+    const T* const v = static_cast<const T*>(p.v_new) + r.first * p.v_st + h * p.v_sh + col;
+    if (lane == 0) first[0][col] = first[1][col] = first[2][col] = kNever;
+    __syncthreads();
+    int f[3] = {kNever, kNever, kNever};
 #pragma unroll 8
-      for (int j = 0; j < r.count; ++j) {
-        const float y = static_cast<float>(v[j * p.v_st]);
-        if (fabsf(y) < INFINITY) continue;
-        for (int i = p.mask ? 0 : j; i < r.count; ++i) {
-          if (p.mask && p.mask[(r.first + i) * p.mask_stride + j]) continue;
-          T* const o = static_cast<T*>(p.o) + (r.first + i) * p.o_st + h * p.group * p.o_sh + col;
-          for (int x = 0; x < p.group; ++x) o[x * p.o_sh] = from_f<T>(static_cast<float>(o[x * p.o_sh]) + y);
-        }
-      }
+    for (int j = lane; j < end; j += kLanes) {
+      const float y = static_cast<float>(v[j * p.v_st]);
+      if (y == INFINITY) f[0] = min(f[0], j);
+      if (y == -INFINITY) f[1] = min(f[1], j);
+      if (y != y) f[2] = min(f[2], j);
     }
+#pragma unroll
+    for (int x = 0; x < 3; ++x)
+      if (f[x] != kNever) atomicMin(&first[x][col], f[x]);
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 3; ++x) f[x] = first[x][col];
+    const int start = min(min(f[0], f[1]), f[2]);
+    const unsigned kinds = (f[0] < kNever ? 1u : 0u) | (f[1] < kNever ? 2u : 0u) | (f[2] < kNever ? 4u : 0u);
+    for (int i = lo + lane; i < hi && kinds; i += kLanes) {
+      unsigned seen = 0;
+      if (p.mask) {
+        const uint8_t* const row = p.mask + (r.first + i) * p.mask_stride;
+        for (int j = start; j < end && seen != kinds && !(seen & 4u); ++j) {
+          if (row[j]) continue;
+          const float y = static_cast<float>(v[j * p.v_st]);
+          seen |= (y == INFINITY ? 1u : 0u) | (y == -INFINITY ? 2u : 0u) | (y != y ? 4u : 0u);
+        }
+      } else {
+        seen = (i >= f[0] ? 1u : 0u) | (i >= f[1] ? 2u : 0u) | (i >= f[2] ? 4u : 0u);
+      }
+      if (!seen) continue;
+      const float y = seen == 1u ? INFINITY : seen == 2u ? -INFINITY : __int_as_float(0x7fc00000);
+      T* const o = static_cast<T*>(p.o) + (r.first + i) * p.o_st + h * p.group * p.o_sh + col;
+      for (int x = 0; x < p.group; ++x) o[x * p.o_sh] = from_f<T>(static_cast<float>(o[x * p.o_sh]) + y);
+    }
+    __syncthreads();
   }
 }
 

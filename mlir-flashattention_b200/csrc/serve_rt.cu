@@ -643,8 +643,13 @@ int launch_tree_hidden(const AttnTree& d, const attn_tree::Params& p, const rt_h
   e = launch_early(clean, dim3(blocks), kThreads, 0, s, p, reinterpret_cast<uint4*>(static_cast<char*>(base) + flags),
                    odd);
   const int rc = e == cudaSuccess ? launch_tree(c, p, dev, s) : ATTN_OK;
-  if (e == cudaSuccess && rc == ATTN_OK)
-    e = launch_early(whole, dim3((d.Hkv * D + kThreads - 1) / kThreads), kThreads, 0, s, p, odd, blocks);
+  if (e == cudaSuccess && rc == ATTN_OK) {
+    // At most 16 blocks go over a request's values of one head.
+    const int rows_each = std::max(128, (p.max_new + 15) / 16), splits = (p.max_new + rows_each - 1) / rows_each;
+    const int64_t items = d.B * d.Hkv * splits;
+    e = launch_early(whole, dim3(static_cast<unsigned>(std::min<int64_t>(items, dev.sms))), kThreads, 0, s, p, odd, blocks,
+                     rows_each, splits);
+  }
   cudaFreeAsync(base, s);
   if (rc != ATTN_OK) return rc;
   if (e != cudaSuccess) return cuda_fail(e, "attn_tree launch");

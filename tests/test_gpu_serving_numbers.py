@@ -113,3 +113,72 @@ def test_rows_that_see_nothing_beside_scores_of_minus_infinity(pkg, dtype, Hq, H
     o, lse = check(pkg, t.run(pkg))
     assert not o[0].any() and not o[3].any() and bool(o[1:3].isnan().all())
     assert bool((lse[:4] == -math.inf).all())
+
+
+def values_definition(t):
+    """O where new values are no numbers: the sum over the finite ones, and by each row and column what the others that
+    the row sees make of it (weights are above 0)."""
+    n = t.rows
+    fine, t.v = t.v, t.v.clone()
+    t.v[:n] = t.v[:n].nan_to_num(0, 0, 0)
+    o, _, a = definition(t)
+    t.v = fine
+    Hq, H = t.q.shape[1], t.v.shape[1]
+    for b in range(len(t.held)):
+        rows = slice(t.starts[b], t.starts[b + 1])
+        m = rows.stop - rows.start
+        seen = torch.ones(m, m, dtype=torch.bool).tril() if t.mask is None else ~t.mask[rows, :m]
+        v = t.v[rows].double()
+        odd = torch.where(v.isfinite(), 0.0, v)
+        for h in range(H):
+            hit = [seen.double() @ kind.double() > 0 for kind in (odd[:, h] == INF, odd[:, h] == -INF, odd[:, h].isnan())]
+            add = hit[0].double().masked_fill(hit[0], INF) + hit[1].double().masked_fill(hit[1], -INF) + \
+                hit[2].double().masked_fill(hit[2], NAN)
+            o[rows, h * (Hq // H):(h + 1) * (Hq // H)] += add[:, None]
+    return o, a
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("mask", [None, "tree", "random"])
+@pytest.mark.parametrize("Hq,H,D,held,new", [(8, 2, 128, [40, 0, 300], [300, 1, 129]), (4, 4, 64, [9000, 5], [7, 160]),
+                                             (5, 1, 128, [0] * 200, [3] * 200)])
+def test_many_values_that_are_no_numbers(pkg, dtype, cache, mask, Hq, H, D, held, new):
+    """Infinities of both signs and NaN in many rows: whole columns, a few a column, both signs in one column."""
+    t = Tree(dtype, cache, Hq, H, 128 if cache is E4M3 else D, 16, held, new, mask, seed=45)
+    g, n = torch.Generator().manual_seed(46), t.rows
+    t.v[:n, :, 0], t.v[:n, 0, 1], t.v[:n, H - 1, 2] = NAN, INF, -INF
+    pick = torch.rand(n, H, generator=g)
+    t.v[:n, :, 3] = torch.where(pick < 0.01, INF, torch.where(pick > 0.99, -INF, 1.0)).to(dtype)
+    t.v[:n, :, 4] = torch.where(pick < 0.3, INF, torch.where(pick > 0.98, NAN, 1.0)).to(dtype)
+    t.v[n - 1, 0, 5], t.v[0, H - 1, 6] = -INF, INF
+    t.run(pkg)
+    pkg.check_status(0)
+    o, a = values_definition(t)
+    got, u = t.o.cpu().double()[:n], half_step(dtype)
+    fine = o.isfinite()
+    assert torch.equal(got.isnan(), o.isnan()) and torch.equal(got[~fine & ~o.isnan()], o[~fine & ~o.isnan()])
+    tol = u * o.abs() + 1.1 * u * a + 1e-6 * a.amax(-1, keepdim=True)
+    assert bool(((got - o).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("mask", [False, True])
+@pytest.mark.parametrize("what", [NAN, INF])
+def test_a_chunk_of_values_that_are_no_numbers_takes_no_longer(pkg, mask, what):
+    """All values of a chunk of 2048 tokens: milliseconds (an update for every pair of a row and a key it sees, one
+    after another, would take seconds)."""
+    T, Hq, H, D = 2048, 32, 8, 128
+    q, k = (torch.randn(T, h, D, device="cuda").to(BF16) for h in (Hq, H))
+    v = torch.full((T, H, D), what, device="cuda").to(BF16)
+    cache = torch.zeros(1, H, 16, D, dtype=BF16, device="cuda")
+    args = (q, k, v, cache, cache, torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+            torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor([0, T], dtype=torch.int32, device="cuda"), 0.1)
+    hide = torch.ones(T, T, dtype=torch.bool, device="cuda").triu(1) if mask else None
+    pkg.fused_tree(*args, mask=hide)
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    o = pkg.fused_tree(*args, mask=hide)
+    end.record()
+    end.synchronize()
+    pkg.check_status(0)
+    assert bool(o.isnan().all() if what != what else (o == INF).all())
+    assert begin.elapsed_time(end) < 100
