@@ -18,6 +18,7 @@ run empty) is recorded in the runtime's status word, which ``check_status`` rais
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import NamedTuple
@@ -84,9 +85,16 @@ def _native():
     return _module
 
 
-def _on_stream(stream):
-    """The stream as torch's current one, so that what is allocated in a call belongs to it too."""
-    return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream))
+def _on_stream(stream, operand):
+    """The stream (a torch stream or a raw handle, of the operand's device) as torch's current one, so that what is
+    allocated in a call belongs to it too."""
+    device = getattr(operand, "device", None)
+    if device is None or device.type != "cuda":
+        return contextlib.nullcontext()  # which the call refuses
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    _need(stream.device == device, f"stream must belong to {device} (got one of {stream.device})")
+    return torch.cuda.stream(stream)
 
 
 def _need(ok, message):
@@ -120,7 +128,7 @@ def cache_plan(lengths, targets, block_table, free_pages, free_count, page_size,
     ATTN_ERR_CAPACITY (ATTN_ERR_INVALID for a length that cannot be).
     """
     if stream is not None:
-        with _on_stream(stream):
+        with _on_stream(stream, lengths):
             return cache_plan(lengths, targets, block_table, free_pages, free_count, page_size, tokens,
                               lengths_out=lengths_out, free_count_out=free_count_out, slots=slots,
                               positions=positions, starts=starts)
@@ -137,7 +145,7 @@ def cache_append(k, v, k_cache, v_cache, slots, *, rows=None, k_descale=1.0, v_d
     cache holds x / descale, saturated to +-448; a descale is a number or an f32 tensor [Hkv].
     """
     if stream is not None:
-        with _on_stream(stream):
+        with _on_stream(stream, k):
             return cache_append(k, v, k_cache, v_cache, slots, rows=rows, k_descale=k_descale, v_descale=v_descale)
     (_module or _native()).append(k, v, k_cache, v_cache, slots, rows, k_descale, v_descale)
 
@@ -207,7 +215,7 @@ def rotary(q, k, positions, freqs, axes=None, *, neighbours=False, inverse=False
     if isinstance(freqs, RotaryTable):
         freqs, axes, neighbours = freqs
     if stream is not None:
-        with _on_stream(stream):
+        with _on_stream(stream, k if q is None else q):
             return _apply_rotary(q, k, positions, freqs, axes, neighbours, inverse)
     return _apply_rotary(q, k, positions, freqs, axes, neighbours, inverse)
 
@@ -233,7 +241,7 @@ def fused_tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, 
     ``output`` may be q itself, but must not overlap the other operands.
     """
     if stream is not None:
-        with _on_stream(stream):
+        with _on_stream(stream, q):
             return fused_tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, scale, mask=mask,
                               max_new=max_new, output=output, lse=lse, k_descale=k_descale, v_descale=v_descale)
     return (_module or _native()).tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, scale, mask, max_new,
