@@ -112,10 +112,15 @@ T* ints(const Tensor& t, const char* name, Ints shape, c10::Device d) {
   return static_cast<T*>(t.data_ptr());
 }
 
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+
 void no_grad(const char* what, std::initializer_list<const Tensor*> list) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const Tensor* t : list)
-    if (t->requires_grad()) refuse(what, " has no backward pass: call it under torch.no_grad()");
+  for (const Tensor* t : list) {
+    if (!t) continue;
+    if (c10::GradMode::is_enabled() && t->requires_grad())
+      refuse(what, " has no backward pass: call it under torch.no_grad()");
+    if (has_tangent(*t)) refuse(what, " has no forward-mode derivative");
+  }
 }
 
 int code_of(at::ScalarType t) {
@@ -132,6 +137,8 @@ int code_of(at::ScalarType t) {
 Tensor empty(Ints shape, at::ScalarType type, c10::Device d) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(d));
 }
+
+const Tensor* maybe(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 // Runs an entry on the current stream of `d`.
 template <typename F, typename D>
@@ -266,7 +273,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse("k and v must both be bfloat16 or both float16");
     if (k.stride(2) != 1 || v.stride(2) != 1) refuse("head_dim must be unit-stride");
     check_cache(kc, vc, H, D, code, d);
-    no_grad("cache_append", {&k, &v});
+    no_grad("cache_append", {&k, &v, &kc, &vc, maybe(a[6]), maybe(a[7])});
     AttnCacheAppend p{};
     p.flags = ATTN_FLAG_DEVICE_POINTERS;
     p.dtype = code;
@@ -377,6 +384,15 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Whether Q or K carries a forward-mode tangent.
+PyObject* dual(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need_count(n, 2);
+    const Tensor *q = maybe(a[0]), *k = maybe(a[1]);
+    return Py_NewRef((q && has_tangent(*q)) || (k && has_tangent(*k)) ? Py_True : Py_False);
+  });
+}
+
 // ----------------------------------------------------------------- attention
 PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -420,7 +436,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.mask = static_cast<const uint8_t*>(mask->data_ptr());
       p.mask_stride = T > 1 ? mask->stride(0) : mask->size(1);
     }
-    no_grad("fused_tree", {&q, &k, &v});
+    no_grad("fused_tree", {&q, &k, &v, &kc, &vc, maybe(a[8]), maybe(a[11]), maybe(a[12]), maybe(a[13]), maybe(a[14])});
     Tensor out;
     if (const Tensor* o = optional_tensor(a[11], "output")) {
       if (o->sizes() != q.sizes() || o->scalar_type() != q.scalar_type() || o->stride(2) != 1)
@@ -474,7 +490,7 @@ PyMethodDef method(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
 }
 
-PyMethodDef g_methods[] = {method<plan>("plan"), method<append>("append"), method<rotate>("rotate"),
+PyMethodDef g_methods[] = {method<plan>("plan"), method<append>("append"), method<rotate>("rotate"), method<dual>("dual"),
                            method<tree>("tree"), {"setup", setup, METH_VARARGS, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 

@@ -142,7 +142,8 @@ def cache_append(k, v, k_cache, v_cache, slots, *, rows=None, k_descale=1.0, v_d
 
     Row ``rows[i]`` (int32 [N]; row i itself when None) goes to slot ``slots[i]`` (int64 [N], as
     :func:`cache_plan` makes them); a slot of -1 takes nothing.  Slots must differ.  A float8_e4m3fn
-    cache holds x / descale, saturated to +-448; a descale is a number or an f32 tensor [Hkv].
+    cache holds x / descale, saturated to +-448; a descale is a number or an f32 tensor [Hkv].  Operands
+    that require a gradient, or carry a forward-mode tangent, are refused.
     """
     if stream is not None:
         with _on_stream(stream, k):
@@ -181,9 +182,21 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, freqs, axes, neighbours, inverse):
         ctx.save_for_backward(positions, freqs, axes)
+        ctx.save_for_forward(positions, freqs, axes)
         ctx.how = neighbours, inverse
         ctx.set_materialize_grads(False)
-        return _native().rotate(q, k, positions, freqs, axes, neighbours, inverse)
+        out = (_module or _native()).rotate(q, k, positions, freqs, axes, neighbours, inverse)
+        ctx.form = [None if x is None else (x.shape, x.dtype, x.device) for x in out]
+        return out
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        """Tangents turn as the values do; an operand without one has the tangent 0."""
+        positions, freqs, axes = ctx.saved_tensors
+        tq, tk = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (tq, tk))
+        turned = _apply_rotary(tq, tk, positions, freqs, axes, *ctx.how)
+        return tuple(torch.zeros(f[0], dtype=f[1], device=f[2]) if t is None and f else t
+                     for t, f in zip(turned, ctx.form))
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -196,9 +209,11 @@ class _Rotary(torch.autograd.Function):
 
 
 def _apply_rotary(q, k, positions, freqs, axes, neighbours, inverse):
-    if ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+    native = _module or _native()
+    if (((q is not None and q.requires_grad) or (k is not None and k.requires_grad)) and torch.is_grad_enabled()) \
+            or native.dual(q, k):
         return _Rotary.apply(q, k, positions, freqs, axes, neighbours, inverse)
-    return (_module or _native()).rotate(q, k, positions, freqs, axes, neighbours, inverse)
+    return native.rotate(q, k, positions, freqs, axes, neighbours, inverse)
 
 
 def rotary(q, k, positions, freqs, axes=None, *, neighbours=False, inverse=False, stream=None):
@@ -210,7 +225,8 @@ def rotary(q, k, positions, freqs, axes=None, *, neighbours=False, inverse=False
     [axes, batch, tokens]; [tokens] for a single axis).  ``freqs`` [dim/2] float64 and ``axes``
     [dim/2] int32 come from :func:`rotary_table` (a whole table may stand in their place).  Pairs are
     (i, i + dim/2), or (2i, 2i + 1) with ``neighbours``; values behind them are copied.  ``inverse``
-    turns back.  Returns the turned (q, k); differentiable in both.
+    turns back.  Returns the turned (q, k); differentiable in both, backward and by forward-mode tangents
+    (``torch.autograd.forward_ad``; the transforms of ``torch.func`` are refused).
     """
     if isinstance(freqs, RotaryTable):
         freqs, axes, neighbours = freqs
@@ -238,7 +254,8 @@ def fused_tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, 
     itself and those before it: a decoded token, or a chunk of a prompt.  ``max_new`` bounds the new
     tokens of a request (default T).  A row that sees nothing gets O = 0 and LSE = -inf; rows past
     ``starts[B]`` are left as they were.  ``lse`` (f32 [T, Hq]) receives the natural-log sums.
-    ``output`` may be q itself, but must not overlap the other operands.
+    ``output`` may be q itself, but must not overlap the other operands.  There is no backward pass:
+    operands that require a gradient, or carry a forward-mode tangent, are refused.
     """
     if stream is not None:
         with _on_stream(stream, q):

@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_serving import BF16, Tree, ints
+from test_gpu_serving import BF16, F32, Tree, check_rotary, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,51 @@ def test_calls_on_a_raw_stream_handle(pkg):
     s.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(again, fused)
     assert torch.equal(o[:t.rows], t.o[:t.rows])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_tangents_of_a_turn(pkg, dtype):
+    """The map is linear: the tangent is the turned tangent."""
+    T, D = 33, 64
+    table, pos = pkg.rotary_table(48, [12, 12]), torch.randint(0, 5000, (2, T), device="cuda")
+    q, k, tq, tk = (torch.randn(T, h, D, device="cuda").to(dtype) for h in (3, 2, 3, 2))
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        a, b = pkg.rotary(fw.make_dual(q, tq), fw.make_dual(k, tk), pos, table)
+        check_rotary(pkg, tq, fw.unpack_dual(a).tangent, pos, table)
+        check_rotary(pkg, tk, fw.unpack_dual(b).tangent, pos, table)
+        check_rotary(pkg, q, fw.unpack_dual(a).primal, pos, table)
+        a, b = pkg.rotary(q, fw.make_dual(k, tk.mT.contiguous().mT), pos, table)  # a tangent of other strides
+        check_rotary(pkg, tk, fw.unpack_dual(b).tangent, pos, table)
+    with pytest.raises(RuntimeError, match="setup_context"):
+        torch.func.jvp(lambda x: pkg.rotary(x, None, pos, table)[0], (q,), (tq,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: pkg.rotary(x, None, pos, table)[0])(q[None])
+    pkg.check_status(0)
+
+
+def test_derivatives_that_are_refused(pkg):
+    """No operand's gradient or tangent is dropped in silence."""
+    t = Tree(BF16, BF16, 2, 1, 64, 16, [5], [1], tail=0)
+    ops = [x.cuda().nan_to_num(0) for x in (t.q, t.k, t.v, t.kc, t.vc)]
+    rest = (t.table.cuda(), ints(t.held), ints(t.starts), 1.0)
+    slots = ints([3], torch.int64)
+    fw = torch.autograd.forward_ad
+    for i in range(5):
+        other = list(ops)
+        other[i] = ops[i].clone().requires_grad_()
+        with pytest.raises(pkg.VerifyError, match="no backward"):
+            pkg.fused_tree(*other, *rest)
+        if i:
+            with pytest.raises(pkg.VerifyError, match="no backward"):
+                pkg.cache_append(*other[1:], slots)
+        with torch.no_grad():
+            pkg.fused_tree(*other, *rest)
+        with fw.dual_level(), torch.no_grad():
+            other[i] = fw.make_dual(ops[i], torch.ones_like(ops[i]))
+            with pytest.raises(pkg.VerifyError, match="forward-mode"):
+                pkg.fused_tree(*other, *rest)
+            if i:
+                with pytest.raises(pkg.VerifyError, match="forward-mode"):
+                    pkg.cache_append(*other[1:], slots)
+    pkg.check_status(0)

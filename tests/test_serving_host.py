@@ -14,6 +14,9 @@ class Recorder:
     def __init__(self):
         self.calls, self.stream = [], None
 
+    def dual(self, q, k):
+        return False
+
     def __getattr__(self, name):
         def call(*args):
             self.calls.append((name, self.stream))
@@ -76,3 +79,73 @@ def test_a_stream_of_another_device_is_refused(pkg, native, name):
 def test_host_operands_reach_the_checks_of_the_call(pkg, native):
     calls(pkg, operand("cpu"), 0x1234)["tree"]()
     assert native.calls == [("tree", None)]
+
+
+# ------------------------------------------------------------------ derivatives of the turn
+@pytest.fixture
+def turning(pkg, monkeypatch):
+    """The native module's turn on CPU tensors, by the plain statement, with its own look for tangents."""
+    import serving_ref as ref
+    pkg.rotary  # noqa: B018
+
+    class Module:
+        dual = staticmethod(pkg.serving._native().dual)
+
+        def rotate(self, q, k, positions, freqs, axes, neighbours, inverse):
+            return tuple(None if x is None else ref.rotary(x, positions, freqs, axes, neighbours, inverse).to(x.dtype)
+                         for x in (q, k))
+
+    monkeypatch.setattr(pkg.serving, "_module", Module())
+    return lambda q, k, pos, table, **kw: pkg.rotary(q, k, pos, table, **kw)
+
+
+def operands(T=6, D=10, dtype=torch.float64):
+    g = torch.Generator().manual_seed(3)
+    q, k, tq, tk = (torch.randn(T, h, D, generator=g, dtype=dtype) for h in (3, 2, 3, 2))
+    return q, k, tq, tk, torch.arange(2 * T).view(2, T) * 5
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_tangents_turn_as_the_values_do(pkg, turning, neighbours, inverse):
+    q, k, tq, tk, pos = operands()
+    table = pkg.rotary_table(8, [2, 2], neighbours=neighbours, device="cpu")
+    want = turning(tq, tk, pos, table, inverse=inverse)
+    values = turning(q, k, pos, table, inverse=inverse)
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        a, b = turning(fw.make_dual(q, tq), fw.make_dual(k, tk), pos, table, inverse=inverse)
+        for x, value, t in ((a, values[0], want[0]), (b, values[1], want[1])):
+            assert torch.equal(fw.unpack_dual(x).primal, value) and torch.equal(fw.unpack_dual(x).tangent, t)
+        # one operand has a tangent, the other none (or is not there, or wants a gradient)
+        a, none = turning(fw.make_dual(q, tq), None, pos, table, inverse=inverse)
+        assert none is None and torch.equal(fw.unpack_dual(a).tangent, want[0])
+        a, b = turning(q, fw.make_dual(k, tk), pos, table, inverse=inverse)
+        assert torch.equal(fw.unpack_dual(b).tangent, want[1])
+        left = fw.unpack_dual(a).tangent
+        assert left is None or not left.any()
+        wants = q.clone().requires_grad_()
+        a, b = turning(wants, fw.make_dual(k, tk), pos, table, inverse=inverse)
+        assert torch.equal(fw.unpack_dual(b).tangent, want[1])
+        with torch.no_grad():
+            a, _ = turning(fw.make_dual(q, tq), None, pos, table, inverse=inverse)
+            assert torch.equal(fw.unpack_dual(a).tangent, want[0])
+
+
+def test_derivatives_against_differences(pkg, turning):
+    q, k, _, _, pos = operands(3)
+    table = pkg.rotary_table(8, [3, 1], device="cpu")
+    q.requires_grad_(), k.requires_grad_()
+    run = lambda a, b: turning(a, b, pos, table)  # noqa: E731
+    assert torch.autograd.gradcheck(run, (q, k), check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(run, (q, k), check_fwd_over_rev=True)
+
+
+def test_transforms_are_refused_not_ignored(pkg, turning):
+    q, _, tq, _, pos = operands()
+    table = pkg.rotary_table(8, device="cpu")
+    run = lambda x: turning(x, None, pos[:1], table)[0]  # noqa: E731
+    with pytest.raises(RuntimeError, match="setup_context"):
+        torch.func.jvp(run, (q,), (tq,))
+    with pytest.raises(RuntimeError, match="setup_context"):
+        torch.func.grad(lambda x: run(x).sum())(q)
