@@ -243,10 +243,14 @@ def fused(Q, K, V, scale, mask=None, output=None, *, causal=False, lse=None,
     ``rotary`` (a ``RotaryTable``) turns Q and K by ``positions`` (int32 or
     int64 [axes, N] or [axes, B, N]) before they meet, on the same stream; Q
     and K then have the same N and neither is e4m3.
+
+    There is no backward pass: the result has no graph.  With ``rotary``, whose
+    own call is differentiable, operands that require a gradient or carry a
+    forward-mode tangent are refused.
     """
     import torch  # noqa: PLC0415
     if rotary is not None or positions is not None:
-        Q, K = _turned(Q, K, rotary, positions, stream)
+        Q, K = _turned(Q, K, V, rotary, positions, stream)
     q4 = _as4(Q, "Q", "seq_q", "head_dim")
     k4 = _as4(K, "K", "seq_k", "head_dim")
     v4 = _as4(V, "V", "seq_k", "head_dim")
@@ -332,10 +336,16 @@ def fused(Q, K, V, scale, mask=None, output=None, *, causal=False, lse=None,
     return output
 
 
-def _turned(Q, K, table, positions, stream):
+def _turned(Q, K, V, table, positions, stream):
     """Q and K of ``fused`` turned by their rotary positions."""
+    import torch  # noqa: PLC0415
     if table is None or positions is None:
         raise VerifyError("rotary and positions go together")
+    if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad):
+        raise VerifyError("fused has no backward pass: call it under torch.no_grad()")
+    dual = _serving()._native().dual
+    if dual(Q, K) or dual(V, None):
+        raise VerifyError("fused has no forward-mode derivative")
     q4, k4 = _as4(Q, "Q", "seq_q", "head_dim"), _as4(K, "K", "seq_k", "head_dim")
     if q4.shape[2] != k4.shape[2]:
         raise VerifyError("rotary positions need K seq_len equal to Q seq_len")

@@ -149,3 +149,19 @@ def test_transforms_are_refused_not_ignored(pkg, turning):
         torch.func.jvp(run, (q,), (tq,))
     with pytest.raises(RuntimeError, match="setup_context"):
         torch.func.grad(lambda x: run(x).sum())(q)
+
+
+def test_fused_with_a_turn_refuses_what_it_cannot_differentiate(pkg):
+    """Before anything else is looked at: a gradient that never arrives is worse than an error."""
+    table, pos = pkg.rotary_table(8, device="cpu"), torch.arange(4)
+    fw = torch.autograd.forward_ad
+    for i in range(3):
+        x = [torch.randn(4, 8) for _ in range(3)]
+        x[i].requires_grad_()
+        with pytest.raises(pkg.VerifyError, match="fused has no backward"):
+            pkg.fused(*x, 0.1, rotary=table, positions=pos)
+        with torch.no_grad(), pytest.raises(pkg.VerifyError, match="CUDA"):
+            pkg.fused(*x, 0.1, rotary=table, positions=pos)
+        x[i] = x[i].detach()
+        with fw.dual_level(), pytest.raises(pkg.VerifyError, match="fused has no forward-mode"):
+            pkg.fused(*(fw.make_dual(y, y) if j == i else y for j, y in enumerate(x)), 0.1, rotary=table, positions=pos)
