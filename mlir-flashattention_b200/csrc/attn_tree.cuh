@@ -57,12 +57,15 @@ struct Request {
 };
 
 // What the device arrays say of request b, cut to what can be read: a length
-// past the table or rows past q would leave the buffers.
+// past the table or rows past q would leave the buffers.  Plain loads, here and
+// wherever a kernel reads what the one before it in the stream may write: these
+// kernels begin before that one ends, so to them such memory is not constant,
+// and a load through the read-only path might be moved above the wait.
 __device__ __forceinline__ Request request(const Params& p, int b) {
   Request r;
-  r.held = __ldg(p.lengths + b);
-  r.first = __ldg(p.starts + b);
-  r.count = __ldg(p.starts + b + 1) - r.first;
+  r.held = p.lengths[b];
+  r.first = p.starts[b];
+  r.count = p.starts[b + 1] - r.first;
   const int most = p.W << p.page_shift;
   if (r.held < 0 || r.held > most || r.count < 0 || r.count > p.max_new || r.first < 0 ||
       r.first > p.T - r.count) {
@@ -364,19 +367,19 @@ constexpr int kValueThreads = 256;
 // odd[block]: whether the block met such a value.
 template <typename T, int D>
 __global__ void __launch_bounds__(kValueThreads)
-    clean_values(const __grid_constant__ Params p, uint4* __restrict__ out, int* __restrict__ odd) {
+    clean_values(const __grid_constant__ Params p, uint4* out, int* odd) {
   constexpr uint32_t kExponent = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
   constexpr int kPacks = D / 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t live = __ldg(p.starts + p.B);  // rows behind them may hold anything
+  const int64_t live = p.starts[p.B];  // rows behind them may hold anything
   const int64_t n = static_cast<int64_t>(p.T) * p.Hkv * kPacks;
   uint32_t met = 0;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kValueThreads) + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * kValueThreads) {
     const int64_t row = i / kPacks;
     const T* const v = static_cast<const T*>(p.v_new) + row / p.Hkv * p.v_st + row % p.Hkv * p.v_sh;
-    uint4 w = __ldg(reinterpret_cast<const uint4*>(v) + i % kPacks);
+    uint4 w = reinterpret_cast<const uint4*>(v)[i % kPacks];
     uint32_t* const x = &w.x;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       };
       auto page_of = [&](int k) {  // of this lane's segment
         if (k >= min(pc.cached, pc.k1) || lane >= segments(k)) return 0;
-        return __ldg(row + (((k << split.keys_shift) + (lane << seg_shift)) >> p.page_shift));
+        return row[((k << split.keys_shift) + (lane << seg_shift)) >> p.page_shift];
       };
       int page_next = page_of(pc.k0);
       for (int k = pc.k0; k < pc.k1 && ok; ++k, ++n) {
@@ -271,20 +271,27 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     const int row0 = pc.rt * C::kRows;  // the item's first row in the request
     const int rows = static_cast<int>(
         min(static_cast<int64_t>(C::kRows), static_cast<int64_t>(pc.r.count) * p.group - row0));
-    // q rows to shared memory (rows behind the last: zeros), 8 threads a row.
+    // q rows to shared memory (rows behind the last: zeros), 8 threads a row; all
+    // loads before the first store.
+    uint4 q_in[MT][D / 64];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int r = 16 * mt + (tid >> 3), at = row0 + r;
       const T* const src = static_cast<const T*>(p.q) + static_cast<int64_t>(pc.r.first + at / p.group) * p.q_st +
                            (pc.h * p.group + at % p.group) * p.q_sh;
-      uint4 v[D / 64];
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        const int chunk = (tid & 7) + 8 * c;
-        v[c] = make_uint4(0, 0, 0, 0);
-        if (r < rows) v[c] = __ldg(reinterpret_cast<const uint4*>(src) + chunk);
-        *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((chunk ^ (r & 7)) * 16)) = v[c];
+        q_in[mt][c] = make_uint4(0, 0, 0, 0);
+        if (r < rows) q_in[mt][c] = reinterpret_cast<const uint4*>(src)[(tid & 7) + 8 * c];
       }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = 16 * mt + (tid >> 3);
+      const uint4 (&v)[D / 64] = q_in[mt];
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        *reinterpret_cast<uint4*>(s_q + r * D * 2 + ((((tid & 7) + 8 * c) ^ (r & 7)) * 16)) = v[c];
       if constexpr (FP8 && !F16) {
         float top = 0.f;
 #pragma unroll
@@ -336,8 +343,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     float kd = scale2, vd = 1.f;
     if constexpr (FP8) {
-      kd *= p.k_descale * (p.k_descale_heads ? __ldg(p.k_descale_heads + pc.h) : 1.f);
-      vd = p.v_descale * (p.v_descale_heads ? __ldg(p.v_descale_heads + pc.h) : 1.f);
+      kd *= p.k_descale * (p.k_descale_heads ? p.k_descale_heads[pc.h] : 1.f);
+      vd = p.v_descale * (p.v_descale_heads ? p.v_descale_heads[pc.h] : 1.f);
     }
     float o[MT][kTilesD][4];
     float m[MT][2], l[MT][2];

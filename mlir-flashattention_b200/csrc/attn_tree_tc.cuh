@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto segments = [&](int k) { return (j.here(split, k) + (1 << seg_shift) - 1) >> seg_shift; };
         auto page_of = [&](int k) {  // of this lane's segment
           if (k >= min(j.cached, j.k1) || lane >= segments(k)) return 0;
-          return __ldg(row + (((k << split.keys_shift) + (lane << seg_shift)) >> p.page_shift));
+          return row[((k << split.keys_shift) + (lane << seg_shift)) >> p.page_shift];
         };
         // K and V of a tile share its page ids, which are read a tile ahead.
         constexpr int kLag = ALONE ? 1 : 0;

@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_serving import BF16, F32, Tree, check_rotary, ints
+from test_gpu_serving import BF16, E4M3, F32, Tree, check_rotary, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -79,4 +79,72 @@ def test_derivatives_that_are_refused(pkg):
             if i:
                 with pytest.raises(pkg.VerifyError, match="forward-mode"):
                     pkg.cache_append(*other[1:], slots)
+    pkg.check_status(0)
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("Hq,H,new,tree", [(8, 8, 1, False), (8, 8, 12, True), (32, 1, 20, True), (16, 2, 40, False)])
+def test_calls_back_to_back(pkg, cache, Hq, H, new, tree):
+    """A step's calls for many layers without a pause, each reading at once what the one before wrote - q and the new
+    keys and values, the lengths, tables and starts of the plan, the pages: the same bits as with a wait after each, and
+    from a captured graph."""
+    B, D, page, pages, layers = 3, 128, 16, 200, 6
+    table = pkg.rotary_table(D)
+    d = 1.0 if cache is BF16 else 0.05
+    g = torch.Generator(device="cuda").manual_seed(52)
+    T = B * new
+    x0 = torch.randn(T, Hq, D, generator=g, device="cuda").to(BF16)
+    kv = [torch.randn(T, H, D, generator=g, device="cuda").to(BF16) for _ in range(2)]
+    filled = [torch.randn(pages, H, page, D, generator=g, device="cuda").to(cache) for _ in range(2)]
+    mask = torch.rand(T, new, generator=g, device="cuda") < 0.5 if tree else None
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+
+    def fresh():
+        blocks = torch.full((B, 60), -1, dtype=torch.int32, device="cuda")
+        held = [700, 5, 16]
+        at = 0
+        for b, n in enumerate(held):
+            blocks[b, :-(-n // page)] = order[at:at - (-n // page)]
+            at -= -n // page
+        free = torch.cat([order[at:], order.new_full((at,), -1)])
+        return [x.clone() for x in filled], ints(held), blocks, free, ints([pages - at]), x0.clone()
+
+    def steps(state, pause):
+        (kc, vc), lengths, blocks, free, count, x = state
+        lse = []
+        for _ in range(2):
+            want = lengths + new
+            plan = pkg.cache_plan(lengths, want, blocks, free, count, page, T)
+            pause()
+            for _ in range(layers):
+                q, k = pkg.rotary(x, kv[0], plan.positions, table)
+                pause()
+                lse.append(torch.empty(T, Hq, device="cuda"))
+                pkg.fused_tree(q, k, kv[1], kc, vc, blocks, lengths, plan.starts, 0.1, mask=mask, max_new=new, output=x,
+                               lse=lse[-1], k_descale=d, v_descale=d)
+                pause()
+                x = pkg.fused_tree(x, k, x[:, :H], kc, vc, blocks, lengths, plan.starts, 0.1, mask=mask, max_new=new,
+                                   k_descale=d, v_descale=d)
+                pause()
+                pkg.cache_append(k, kv[1], kc, vc, plan.slots, k_descale=d, v_descale=d)
+                pause()
+            lengths, count = plan.lengths, plan.free_count
+        return [x, *lse, kc.view(torch.uint8), vc.view(torch.uint8), blocks, free]
+
+    want = steps(fresh(), torch.cuda.synchronize)
+    pkg.check_status(0)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(steps(fresh(), lambda: None), want))
+    state = fresh()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = steps(state, lambda: None)
+    again = fresh()
+    for _ in range(2):
+        for a, b in zip([*state[0], *state[1:]], [*again[0], *again[1:]]):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
     pkg.check_status(0)
