@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   // are complete) before one of them is written.
   cluster.sync();
   const int rank = static_cast<int>(cluster.block_rank());
-  const int step = threads * static_cast<int>(cluster.num_blocks());
+  const int64_t step = threads * static_cast<int>(cluster.num_blocks());  // past 2^31 a step may lead
   const int first = rank * threads + tid;
 
   // Index x of the given-back pages: a table entry past its request's new end.
@@ -171,16 +171,16 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
   const int per = p.tokens > step ? kRun : 1;
   const bool aligned = per == kRun && (reinterpret_cast<uintptr_t>(p.slots) & 15u) == 0 &&
                     (reinterpret_cast<uintptr_t>(p.positions) & 15u) == 0;
-  for (int i0 = first * per; i0 < p.tokens; i0 += step * per) {
+  for (int64_t i0 = first * per; i0 < p.tokens; i0 += step * per) {
     int64_t slot[kRun];
     int position[kRun];
     int b = -1, page = 0, have = 0;
     const int32_t* row = nullptr;
 #pragma unroll
     for (int x = 0; x < kRun; ++x) {
-      const int i = i0 + x;
       slot[x] = -1, position[x] = 0;
-      if (x >= per || i >= total) continue;
+      if (x >= per || i0 + x >= total) continue;
+      const int i = static_cast<int>(i0) + x;
       const bool next = b < 0 || i >= tok_pre[b + 1];
       if (next) {
         if (b < 0) b = owner(tok_pre, p.B, i);
@@ -211,18 +211,18 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Params p) {
       }
     }
   }
-  for (int b = first; b <= p.B; b += step) p.starts[b] = ok ? tok_pre[b] : 0;
+  for (int64_t b = first; b <= p.B; b += step) p.starts[b] = ok ? tok_pre[b] : 0;
   if (ok) {
-    for (int k = first; k < A; k += step) {
-      const int b = owner(grow_pre, p.B, k);
+    for (int64_t k = first; k < A; k += step) {
+      const int b = owner(grow_pre, p.B, static_cast<int>(k));
       const int have = (held[b] + round_up) >> p.page_shift;
-      p.table[b * p.table_stride + have + (k - grow_pre[b])] = popped(k);
+      p.table[b * p.table_stride + have + (k - grow_pre[b])] = popped(static_cast<int>(k));
     }
-    for (int i = F + first; i < F + R - A; i += step) p.free_pages[i] = given_back(i - F);
+    for (int64_t i = int64_t{F} + first; i < F + R - A; i += step) p.free_pages[i] = given_back(static_cast<int>(i) - F);
   }
   // In place where the caller gave the same arrays.  targets may be
   // lengths_out too: then it holds what is written.
-  for (int b = first; b < p.B; b += step) p.lengths_out[b] = ok ? p.targets[b] : held[b];
+  for (int64_t b = first; b < p.B; b += step) p.lengths_out[b] = ok ? p.targets[b] : held[b];
   if (first == 0) {
     *p.free_count_out = ok ? F + R - A : F;
     if (!ok) atomicCAS(p.status, 0, bad ? ATTN_ERR_INVALID : ATTN_ERR_CAPACITY);

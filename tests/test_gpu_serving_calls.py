@@ -148,3 +148,18 @@ def test_calls_back_to_back(pkg, cache, Hq, H, new, tree):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     pkg.check_status(0)
+
+
+def test_plan_with_as_many_tokens_as_there_may_be(pkg):
+    """A padded call of 2^31 - 1 tokens: indexes that step past 2^31 end the loop."""
+    tokens = (1 << 31) - 1
+    blocks, free = ints([[3, -1], [-1, -1]]), ints([9, 8, 7])
+    lengths = ints([10, 0])
+    slots = torch.full((tokens,), 5, dtype=torch.int64, device="cuda")
+    plan = pkg.cache_plan(lengths, ints([20, 5]), blocks, free, ints([3]), 16, tokens, slots=slots)
+    pkg.check_status(0)
+    want = [58, 59, 60, 61, 62, 63, 112, 113, 114, 115, 128, 129, 130, 131, 132]  # pages 3 and 7, then 8
+    assert slots[:15].tolist() == want and plan.starts.tolist() == [0, 10, 15]
+    assert plan.positions[:15].tolist() == [*range(10, 20), *range(5)] and blocks.tolist() == [[3, 7], [8, -1]]
+    for at in range(15, tokens, 1 << 28):
+        assert bool((slots[at:at + (1 << 28)] == -1).all()) and not plan.positions[at:at + (1 << 28)].any()
