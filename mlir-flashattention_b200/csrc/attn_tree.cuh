@@ -106,7 +106,7 @@ __device__ __forceinline__ int new_tiles(const Params& p, const Split& s, const 
 }
 
 __device__ __forceinline__ int cached_tiles(const Split& s, const Request& r) {
-  return (r.held + (1 << s.keys_shift) - 1) >> s.keys_shift;
+  return static_cast<int>((static_cast<uint32_t>(r.held) + (1u << s.keys_shift) - 1) >> s.keys_shift);  // may pass 2^31
 }
 
 __device__ __forceinline__ int row_tiles(const Params& p, const Split& s, const Request& r) {

@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_serving import BF16, E4M3, F32, Tree, check_rotary, ints
+from test_gpu_serving import BF16, E4M3, F16, F32, Tree, check_rotary, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -163,3 +163,24 @@ def test_plan_with_as_many_tokens_as_there_may_be(pkg):
     assert plan.positions[:15].tolist() == [*range(10, 20), *range(5)] and blocks.tolist() == [[3, 7], [8, -1]]
     for at in range(15, tokens, 1 << 28):
         assert bool((slots[at:at + (1 << 28)] == -1).all()) and not plan.positions[at:at + (1 << 28)].any()
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_a_request_as_long_as_there_may_be(pkg, new):
+    """2^31 - 16 cached tokens, one page over and over: the number of key tiles is taken past 2^31.
+
+    Each of a share's four warps (60 rows: each share's two accumulators) adds 2^31 / (296 * 4) keys, 16 to 128 at a
+    time, one after another in 32 bits: 1.2e5 additions off by 2^-23 of the sum at most in the products, 4 a lane in the
+    weights: 4.6e5 by 2^-24, below 3 % in all, of both the sums that O divides; 0.03 in LSE."""
+    W, page, D = (1 << 27) - 1, 16, 64
+    g = torch.Generator().manual_seed(53)
+    q, k, v = (torch.randn(new, 1, D, generator=g).to(F16) for _ in range(3))
+    kc, vc = (torch.randn(1, 1, page, D, generator=g).to(F16) for _ in range(2))
+    o, lse = torch.empty(new, 1, D, dtype=F16, device="cuda"), torch.empty(new, 1, device="cuda")
+    pkg.fused_tree(q.cuda(), k.cuda(), v.cuda(), kc.cuda(), vc.cuda(), torch.zeros(1, W, dtype=torch.int32, device="cuda"),
+                   ints([W * page]), ints([0, new]), 0.1, max_new=new, output=o, lse=lse)
+    pkg.check_status(0)
+    s = q[:, 0].double() @ kc[0, 0].double().T * 0.1  # the new keys weigh 2^-27 of these
+    want, size = torch.softmax(s, 1) @ vc[0, 0].double(), torch.softmax(s, 1) @ vc[0, 0].double().abs()
+    assert bool(((o.cpu().double()[:, 0] - want).abs() <= 0.06 * size).all())
+    assert bool(((lse.cpu().double()[:, 0] - torch.logsumexp(s, 1) - 27 * 0.6931471805599453).abs() <= 0.03).all())
