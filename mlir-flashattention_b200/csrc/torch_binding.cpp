@@ -33,6 +33,21 @@ struct Failed {  // becomes AttentionError
 };
 struct Raised {};  // a Python error is set
 
+// The interpreter's lock, given up while memory is allocated and kernels are
+// launched: with a full launch queue either may wait for the GPU, which in turn
+// may wait for what another Python thread has yet to do.  Nothing in such a
+// scope touches Python objects.
+class Unlocked {
+ public:
+  Unlocked() : state_(PyEval_SaveThread()) {}
+  ~Unlocked() { PyEval_RestoreThread(state_); }
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+
+ private:
+  PyThreadState* state_;
+};
+
 PyObject* g_verify_error = nullptr;
 PyObject* g_attention_error = nullptr;
 decltype(&attn_cache_plan) g_plan = nullptr;
@@ -199,19 +214,22 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.block_table = static_cast<int32_t*>(table.data_ptr());
     p.free_pages = ints(free_pages, "free_pages", {p.num_pages}, d);
     p.free_count = ints(free_count, "free_count", {1}, d);
-    auto out = [&](int i, const char* name, int64_t size, at::ScalarType type) {
-      const Tensor* t = optional_tensor(a[i], name);
-      return t ? *t : empty({size}, type, d);
-    };
-    const Tensor lengths_out = out(7, "lengths_out", B, at::kInt), count_out = out(8, "free_count_out", 1, at::kInt),
-                 slots = out(9, "slots", tokens, at::kLong), positions = out(10, "positions", tokens, at::kInt),
-                 starts = out(11, "starts", B + 1, at::kInt);
-    p.lengths_out = ints(lengths_out, "lengths_out", {B}, d);
-    p.free_count_out = ints(count_out, "free_count_out", {1}, d);
-    p.slots = ints<int64_t>(slots, "slots", {tokens}, d);
-    p.positions = ints(positions, "positions", {tokens}, d);
-    p.starts = ints(starts, "starts", {B + 1}, d);
-    launch(g_plan, p, d);
+    constexpr const char* names[5] = {"lengths_out", "free_count_out", "slots", "positions", "starts"};
+    const Tensor* given[5];
+    for (int i = 0; i < 5; ++i) given[i] = optional_tensor(a[7 + i], names[i]);
+    Tensor lengths_out, count_out, slots, positions, starts;
+    {
+      Unlocked unlocked;
+      auto out = [&](int i, int64_t size, at::ScalarType type) { return given[i] ? *given[i] : empty({size}, type, d); };
+      lengths_out = out(0, B, at::kInt), count_out = out(1, 1, at::kInt), slots = out(2, tokens, at::kLong);
+      positions = out(3, tokens, at::kInt), starts = out(4, B + 1, at::kInt);
+      p.lengths_out = ints(lengths_out, names[0], {B}, d);
+      p.free_count_out = ints(count_out, names[1], {1}, d);
+      p.slots = ints<int64_t>(slots, names[2], {tokens}, d);
+      p.positions = ints(positions, names[3], {tokens}, d);
+      p.starts = ints(starts, names[4], {B + 1}, d);
+      launch(g_plan, p, d);
+    }
     PyObject* r = PyTuple_New(5);
     const Tensor* parts[5] = {&slots, &positions, &starts, &lengths_out, &count_out};
     for (int i = 0; r && i < 5; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(*parts[i]));
@@ -285,7 +303,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (rows) p.rows = ints(*rows, "rows", {p.N}, d);
     descale(a[6], "k_descale", H, d, p.k_descale, p.k_descale_heads);
     descale(a[7], "v_descale", H, d, p.v_descale, p.v_descale_heads);
-    launch(g_append, p, d);
+    {
+      Unlocked unlocked;
+      launch(g_append, p, d);
+    }
     Py_RETURN_NONE;
   });
 }
@@ -326,6 +347,8 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.dtype = code_of(type);
     if (p.dtype != ATTN_F32 && p.dtype != ATTN_BF16 && p.dtype != ATTN_F16)
       refuse("rotary takes float32, bfloat16 or float16 (got ", name_of(type), ")");
+    p.neighbours = truth(a[5]);
+    p.inverse = truth(a[6]);
     Tensor q_out, k_out;
     View f{};
     auto operand = [&](const Tensor* x, const char* name, int64_t& heads, int64_t (&stride)[3], int64_t (&out_stride)[3],
@@ -335,7 +358,10 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (x != &first && (v.B != f.B || v.N != f.N || v.D != f.D || x->dim() != first.dim()))
         refuse("Q and K must have the same tokens and head_dim");
       if (x == &first) f = v;
-      out = at::empty_like(*x);
+      {
+        Unlocked unlocked;
+        out = at::empty_like(*x);
+      }
       const View o = view(out, name, d, type);
       heads = v.H;
       for (int i = 0; i < 3; ++i) stride[i] = v.stride[i], out_stride[i] = o.stride[i];
@@ -370,9 +396,10 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (p.num_axes == 0) refuse("positions need an axis");
     p.positions = pos.data_ptr();
-    p.neighbours = truth(a[5]);
-    p.inverse = truth(a[6]);
-    launch(g_rotary, p, d);
+    {
+      Unlocked unlocked;
+      launch(g_rotary, p, d);
+    }
     PyObject* r = PyTuple_New(2);
     if (!r) throw Raised{};
     const Tensor* outs[2] = {q ? &q_out : nullptr, k ? &k_out : nullptr};
@@ -444,6 +471,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
       on_device(*o, "output", d);
       out = *o;
     } else {
+      Unlocked unlocked;
       out = empty({T, Hq, D}, q.scalar_type(), d);
     }
     if (const Tensor* lse = optional_tensor(a[12], "lse")) {
@@ -459,7 +487,10 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.o_stride[i] = out.stride(i);
     }
     p.q = q.data_ptr(), p.k_new = k.data_ptr(), p.v_new = v.data_ptr(), p.o = out.data_ptr();
-    launch(g_tree, p, d);
+    {
+      Unlocked unlocked;
+      launch(g_tree, p, d);
+    }
     return THPVariable_Wrap(out);
   });
 }

@@ -1,5 +1,8 @@
 """GPU: how the serving calls are made - streams, derivatives, calls back to back, extreme sizes."""
 
+import threading
+import time
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -184,3 +187,40 @@ def test_a_request_as_long_as_there_may_be(pkg, new):
     want, size = torch.softmax(s, 1) @ vc[0, 0].double(), torch.softmax(s, 1) @ vc[0, 0].double().abs()
     assert bool(((o.cpu().double()[:, 0] - want).abs() <= 0.06 * size).all())
     assert bool(((lse.cpu().double()[:, 0] - torch.logsumexp(s, 1) - 27 * 0.6931471805599453).abs() <= 0.03).all())
+
+
+@pytest.mark.parametrize("name", ["plan", "append", "rotary", "tree"])
+def test_other_threads_run_while_a_call_waits_for_the_queue(pkg, name):
+    """A call that finds the launch queue full waits for the GPU without the interpreter's lock."""
+    t = Tree(BF16, BF16, 2, 1, 64, 16, [30], [2], None, seed=54, tail=0)
+    q, k, v, kc, vc, blocks = (x.cuda().nan_to_num(0) for x in (t.q, t.k, t.v, t.kc, t.vc, t.table))
+    held, starts, slots, table = ints(t.held), ints(t.starts), ints([16, 17], torch.int64), pkg.rotary_table(64)
+    free, count, pos = ints([0, 1]), ints([2]), ints([3, 4])
+    calls = {"plan": lambda: pkg.cache_plan(held, held, blocks, free, count, 16, 2),
+             "append": lambda: pkg.cache_append(k, v, kc, vc, slots),
+             "rotary": lambda: pkg.rotary(q, k, pos, table),
+             "tree": lambda: pkg.fused_tree(q, k, v, kc, vc, blocks, held, starts, 0.1, max_new=2)}
+    calls[name]()
+    torch.cuda.synchronize()
+    ticks, done = [], threading.Event()
+
+    def tick():
+        while not done.wait(0.001):
+            ticks.append(time.perf_counter())
+
+    other = threading.Thread(target=tick)
+    other.start()
+    try:
+        torch.cuda._sleep(1_500_000_000)  # about 0.8 s
+        begin = time.perf_counter()
+        for _ in range(3000):
+            calls[name]()
+        took = time.perf_counter() - begin
+    finally:
+        done.set()
+        other.join()
+    torch.cuda.synchronize()
+    pkg.check_status(0)
+    assert took > 0.4, "the queue never filled"
+    inside = [x for x in ticks if begin < x < begin + took]
+    assert max(b - a for a, b in zip([begin, *inside], [*inside, begin + took])) < 0.2
