@@ -153,6 +153,13 @@ Tensor empty(Ints shape, at::ScalarType type, c10::Device d) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(d));
 }
 
+// A tensor that was written in place: autograd then knows that what it saved of
+// it is no longer there.
+void written(std::initializer_list<const Tensor*> list) {
+  for (const Tensor* t : list)
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 const Tensor* maybe(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 // Runs an entry on the current stream of `d`.
@@ -230,6 +237,7 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.starts = ints(starts, names[4], {B + 1}, d);
       launch(g_plan, p, d);
     }
+    written({&table, &free_pages, given[0], given[1], given[2], given[3], given[4]});
     PyObject* r = PyTuple_New(5);
     const Tensor* parts[5] = {&slots, &positions, &starts, &lengths_out, &count_out};
     for (int i = 0; r && i < 5; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(*parts[i]));
@@ -307,6 +315,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Unlocked unlocked;
       launch(g_append, p, d);
     }
+    written({&kc, &vc});
     Py_RETURN_NONE;
   });
 }
@@ -491,6 +500,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Unlocked unlocked;
       launch(g_tree, p, d);
     }
+    written({maybe(a[11]), maybe(a[12])});
     return THPVariable_Wrap(out);
   });
 }

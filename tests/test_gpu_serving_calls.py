@@ -224,3 +224,26 @@ def test_other_threads_run_while_a_call_waits_for_the_queue(pkg, name):
     assert took > 0.4, "the queue never filled"
     inside = [x for x in ticks if begin < x < begin + took]
     assert max(b - a for a, b in zip([begin, *inside], [*inside, begin + took])) < 0.2
+
+
+def test_what_a_call_writes_is_known_to_autograd(pkg):
+    """Positions that a turn saved for its gradient and a later plan overwrites: an error, not another gradient."""
+    x, table = torch.randn(2, 1, 64, device="cuda", requires_grad=True), pkg.rotary_table(64)
+    lengths, blocks, free = ints([3]), ints([[1, -1]]), ints([0])
+    plan = pkg.cache_plan(lengths, ints([5]), blocks, free, ints([1]), 16, 2)
+    y, _ = pkg.rotary(x, None, plan.positions, table)
+    pkg.cache_plan(ints([5]), ints([7]), blocks, free, ints([1]), 16, 2, positions=plan.positions)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    t = Tree(BF16, BF16, 2, 1, 64, 16, [5], [1], None, seed=55, tail=0)
+    q, k, v, kc, vc = (z.cuda().nan_to_num(0) for z in (t.q, t.k, t.v, t.kc, t.vc))
+    lse, o = torch.empty(1, 2, device="cuda"), torch.empty_like(q)
+    before = [z._version for z in (q, k, v, kc, vc, o, lse)]
+    pkg.fused_tree(q, k, v, kc, vc, t.table.cuda(), ints(t.held), ints(t.starts), 0.1, output=o, lse=lse)
+    pkg.cache_append(k, v, kc, vc, ints([8], torch.int64))
+    assert [z._version - n for z, n in zip((q, k, v, kc, vc, o, lse), before)] == [0, 0, 0, 1, 1, 1, 1]
+    with torch.inference_mode():  # tensors that count no versions
+        made = [z.clone() for z in (q, k, v, kc, vc)]
+    pkg.cache_append(*made[1:], ints([8], torch.int64))
+    pkg.fused_tree(*made, t.table.cuda(), ints(t.held), ints(t.starts), 0.1, output=made[0])
+    pkg.check_status(0)
