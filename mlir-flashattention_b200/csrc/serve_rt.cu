@@ -63,6 +63,11 @@ bool stride_ok(int64_t stride, int64_t extent, int64_t multiple) {
   return extent <= 1 || stride % multiple == 0;
 }
 
+// Of what a call writes: rows of `row` elements along a stride are apart.
+bool apart(int64_t stride, int64_t extent, int64_t row) {
+  return extent <= 1 || stride >= row || stride <= -row;
+}
+
 int pow2_shift(int64_t n, int lo, int hi) {
   int s = lo;
   while (s < hi && (int64_t{1} << s) < n) ++s;
@@ -187,6 +192,9 @@ int check(const AttnCacheAppend& d) {
   for (const int64_t* st : {d.k_cache_stride, d.v_cache_stride})
     if (!stride_ok(st[0], d.num_pages, ca) || !stride_ok(st[1], d.Hkv, ca) || st[2] % ca != 0)
       return fail(ATTN_ERR_ALIGN, "cache strides must be multiples of 16 bytes");
+  for (const int64_t* st : {d.k_cache_stride, d.v_cache_stride})
+    if (!apart(st[0], d.num_pages, d.D) || !apart(st[1], d.Hkv, d.D) || !apart(st[2], d.page_size, d.D))
+      return fail(ATTN_ERR_STRIDE, "rows of the cache overlap");
   return ATTN_OK;
 }
 
@@ -251,6 +259,10 @@ int check(const AttnRotary& d) {
   const unsigned eb = d.dtype == ATTN_F32 ? 4 : 2;
   for (const void* ptr : {d.q, d.k, static_cast<const void*>(d.qo), static_cast<const void*>(d.ko)})
     if (!aligned(ptr, eb)) return fail(ATTN_ERR_ALIGN, "Q and K must be aligned to their elements");
+  struct { const int64_t* st; int64_t heads; } outs[] = {{d.qo_stride, d.Hq}, {d.ko_stride, d.Hk}};
+  for (const auto& o : outs)
+    if (o.heads > 0 && (!apart(o.st[0], d.B, d.D) || !apart(o.st[1], o.heads, d.D) || !apart(o.st[2], d.N, d.D)))
+      return fail(ATTN_ERR_STRIDE, "rows of the results overlap");
   return ATTN_OK;
 }
 
@@ -373,6 +385,8 @@ int check(const AttnTree& d) {
   for (const int64_t* st : {d.k_cache_stride, d.v_cache_stride})
     if (!stride_ok(st[0], d.num_pages, ca) || !stride_ok(st[1], d.Hkv, ca) || st[2] % ca != 0)
       return fail(ATTN_ERR_ALIGN, "cache strides must be multiples of 16 bytes");
+  if (!apart(d.o_stride[0], d.T, d.D) || !apart(d.o_stride[1], d.Hq, d.D))
+    return fail(ATTN_ERR_STRIDE, "rows of the result overlap");
   return ATTN_OK;
 }
 

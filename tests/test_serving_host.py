@@ -165,3 +165,30 @@ def test_fused_with_a_turn_refuses_what_it_cannot_differentiate(pkg):
         x[i] = x[i].detach()
         with fw.dual_level(), pytest.raises(pkg.VerifyError, match="fused has no forward-mode"):
             pkg.fused(*(fw.make_dual(y, y) if j == i else y for j, y in enumerate(x)), 0.1, rotary=table, positions=pos)
+
+
+# ------------------------------------------------------------------ what a call would write twice
+@pytest.mark.parametrize("kw", [{"k_cache_stride": [0, 1024, 64]}, {"v_cache_stride": [2048, 0, 64]},
+                                {"k_cache_stride": [2048, 1024, 0]}, {"v_cache_stride": [2048, 32, 64]}])
+def test_a_cache_whose_rows_overlap_is_refused(pkg, kw):
+    from test_serving import _append
+    assert _append(pkg, **kw) == -3 and "overlap" in pkg.last_error()
+
+
+@pytest.mark.parametrize("kw", [{"o_stride": [0, 128]}, {"o_stride": [1024, 0]}, {"o_stride": [1024, 64]}])
+def test_a_result_whose_rows_overlap_is_refused(pkg, kw):
+    from test_serving import _tree
+    assert _tree(pkg, **kw) == -3 and "overlap" in pkg.last_error()
+
+
+@pytest.mark.parametrize("strides", [[0, 0, 128], [0, 64, 0], [0, 32, 128]])
+def test_a_turn_whose_rows_overlap_is_refused(pkg, strides):
+    import ctypes
+    for heads, field in (("Hq", "qo_stride"), ("Hk", "ko_stride")):
+        d = pkg.AttnRotary()
+        d.dtype, d.num_axes, d.B, d.N, d.D, d.R = pkg.ATTN_BF16, 1, 1, 4, 64, 64
+        setattr(d, heads, 2)
+        for f in ("q", "k", "qo", "ko", "positions", "freqs"):
+            setattr(d, f, 0x10000)
+        getattr(d, field)[:] = strides
+        assert pkg.lib().attn_rotary(ctypes.byref(d), None) == -3 and "overlap" in pkg.last_error()
