@@ -192,3 +192,14 @@ def test_a_turn_whose_rows_overlap_is_refused(pkg, strides):
             setattr(d, f, 0x10000)
         getattr(d, field)[:] = strides
         assert pkg.lib().attn_rotary(ctypes.byref(d), None) == -3 and "overlap" in pkg.last_error()
+
+
+def test_the_c_library_builds_without_torch():
+    """Its entries need none: only the calls on torch tensors are left out."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mlir-flashattention_b200", "csrc")
+    plans = [subprocess.run(["make", "-C", csrc, "-n", "-B", *more], capture_output=True, text=True, check=True).stdout
+             for more in ([], ["PYTHON=false"])]
+    assert all("libattnrt.so" in x for x in plans)
+    assert "torch_binding.cpp" in plans[0] and "torch_binding.cpp" not in plans[1]
