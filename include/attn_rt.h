@@ -296,7 +296,9 @@ ATTN_API int attn_fwd_host_noalloc(const AttnDesc* desc, void* stream);
  * All calls are asynchronous on `stream` and take device pointers.  Lengths,
  * tables and slots are device data that the host never sees: what is wrong with
  * them is recorded in the status word (`status`, or the runtime's per-device
- * word when null; attn_rt_check_status) and the rows concerned are skipped.
+ * word when null; attn_rt_check_status).  A request whose lengths or rows cannot
+ * be, and a row whose slot cannot be, are skipped; the keys and values of a page
+ * that is not in the cache count as zeros.
  * Calls may be captured into CUDA graphs (after a first call of the kind on the
  * device outside of a capture) and run on several streams at once, as long as
  * the buffers they write differ. */
@@ -415,7 +417,9 @@ typedef struct AttnTree {
   int32_t page_size;
   int64_t B, T, Hq, Hkv, D;
   int64_t W, num_pages;    /* columns of block_table; pages of the cache          */
-  int64_t max_new;         /* no request has more new tokens than this            */
+  int64_t max_new;         /* no request has more new tokens than this; max_new *
+                              Hq / Hkv rows choose the kernel for the whole call:
+                              a bound far too high costs time                     */
   int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2];  /* token, head     */
   int64_t k_cache_stride[3], v_cache_stride[3];                /* page, head, token */
   int64_t table_stride;    /* elements between rows of block_table                */

@@ -359,8 +359,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __
 // There the attention reads a copy of the new values in which such values are
 // 0 (clean_values), and in the end the rows that do see them get them back,
 // where they decide the sum whatever their weights (whole_values).  Two small
-// launches, 8 us of a call (64 drafted tokens for each of 8 requests with
-// 16384 keys: 114 -> 122 us; 2048 for each of 2: 470 -> 484); in the
+// launches, 8 us of a call and a copy of V (64 drafted tokens for each of 8
+// requests with 16384 keys: 114 -> 122 us; 2048 for each of 2: 470 -> 484); in the
 // attention's own loops, whose registers are all taken, the same cost 9 to 120 us.
 constexpr int kValueThreads = 256;
 

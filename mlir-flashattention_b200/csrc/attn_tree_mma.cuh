@@ -15,15 +15,16 @@
 // warp's work).  MT = 1, 2 or (D = 64) 3 16-row tiles share every key that is
 // read; more rows are more items.  From there on the warps' own instructions
 // bound it (64 rows at D = 64 and 8000 keys: 219 us, 212 us in attn_tree_tc.cuh;
-// 128 rows 378 and 214).  64 requests with 8192 keys, 8 kv-heads, bf16: 196 us,
-// 6.1 TB/s.
+// 128 rows 378 and 214).  64 requests with 8192 keys, 8 kv-heads, bf16: 197 to
+// 201 us from one GPU to another, 6.0 to 6.1 TB/s.
 //
 // An e4m3 cache is met in f16: e4m3 values are f16 values, and a bf16 row of q
-// scaled by the power of two that brings its largest value to 2^14..2^15 is
-// exact in f16 down to 2^-39 of that value.  New keys and values are 16-bit
+// is scaled by the power of two that brings its largest value to 2^14..2^15:
+// its 8 bits are then exact in f16 down to 2^-31 of that value, and below that
+// the row is rounded to f16's smallest step, off by at most 2^-39 of it.  New keys and values are 16-bit
 // and met in their own type.  A tile is twice as many keys, so a warp has two
 // groups of 16 at once (MT = 1): the conversions' latency, not their number,
-// was the bound.  100 requests with 8192 keys: 203 us, 4.5 TB/s; the loads
+// was the bound.  100 requests with 8192 keys: 205 us, 4.4 TB/s; the loads
 // alone take 162 us, the readers' instructions are the rest.
 //
 // Weights are rounded to the operands' type for P V.  In bf16 a rounding by

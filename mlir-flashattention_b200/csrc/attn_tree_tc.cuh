@@ -33,9 +33,11 @@
 //
 // What bounds it is the chain of a tile: S read, maximum, exponentials, P
 // written, P V, about 3,850 clocks a pair of tiles while the tensor cores need
-// half: 2048 new tokens on 8192 keys, 64 heads on 8, 2 requests: 470 us, 0.9
-// PFLOP/s.  64 drafted tokens on 16384 keys, 8 requests: 114 us with the mask's
-// bits, 73 us without a mask.
+// half: 2048 new tokens on 8192 keys, 32 heads on 8, 2 requests: 470 us, 0.9
+// PFLOP/s; 484 for the whole call with clean_values and whole_values.  64 drafted
+// tokens on 16384 keys, 8 requests: 114 us with the mask's bits (122 the whole
+// call), 73 us without a mask.  With a mask the kernel spills 164 bytes a thread,
+// without one 12.
 #pragma once
 
 #include "attn_tree_mma.cuh"

@@ -5,7 +5,8 @@
 // moves 16 keys' and 16 values' numbers of one row, four 16-byte loads in flight
 // and stores of 16 bytes, e4m3 rows too.  64 tokens 1.9 us; 16384 tokens into an
 // e4m3 cache 25 us against 14 for the bytes: the exact division is the rest
-// (times the reciprocal 18 us, but not the formula's bits).
+// (the product with the reciprocal alone 18 us, but not the formula's bits; a
+// product that is corrected by its remainder is untried).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -6,7 +6,7 @@
 // of a radian in 32 bits.  Every head of a token shares the angles, so a block
 // forms them once in shared memory; the rest is one read and one write of Q
 // and K, which bounds the kernel: 16384 tokens of 32 + 32 heads of 128 in bf16,
-// there and back, 187 us, 5.7 TB/s (memory alone would be 164).
+// there and back, 192 us, 5.6 TB/s (memory alone would be 164).
 #pragma once
 
 #include <cuda_bf16.h>

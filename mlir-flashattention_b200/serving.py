@@ -252,10 +252,12 @@ def fused_tree(q, k_new, v_new, k_cache, v_cache, block_table, lengths, starts, 
     ``mask`` (bool or uint8 [T, >= max_new], True = masked) says which new tokens of its request a
     row does not see: all but itself and its ancestors for a drafted tree.  Without a mask a row sees
     itself and those before it: a decoded token, or a chunk of a prompt.  ``max_new`` bounds the new
-    tokens of a request (default T).  A row that sees nothing gets O = 0 and LSE = -inf; rows past
-    ``starts[B]`` are left as they were.  ``lse`` (f32 [T, Hq]) receives the natural-log sums.
-    ``output`` may be q itself, but must not overlap the other operands.  There is no backward pass:
-    operands that require a gradient, or carry a forward-mode tangent, are refused.
+    tokens of a request (default T) and chooses the kernel for the whole call, so give it: 1 for a
+    step of decoded tokens, which without it would run as a call for many rows.  A row that sees
+    nothing gets O = 0 and LSE = -inf, one whose scores are no numbers or all -inf an O that is none;
+    rows past ``starts[B]`` are left as they were.  ``lse`` (f32 [T, Hq]) receives the natural-log
+    sums.  ``output`` may be q itself, but must not overlap the other operands.  There is no backward
+    pass: operands that require a gradient, or carry a forward-mode tangent, are refused.
     """
     if stream is not None:
         with _on_stream(stream, q):
