@@ -1,5 +1,6 @@
 """GPU: how the serving calls are made - streams, derivatives, calls back to back, extreme sizes."""
 
+import math
 import threading
 import time
 
@@ -247,3 +248,39 @@ def test_what_a_call_writes_is_known_to_autograd(pkg):
     pkg.cache_append(*made[1:], ints([8], torch.int64))
     pkg.fused_tree(*made, t.table.cuda(), ints(t.held), ints(t.starts), 0.1, output=made[0])
     pkg.check_status(0)
+
+
+def test_threads_call_at_once(pkg):
+    """Each on a stream of its own, refused calls among them: the bits of a call alone, and each thread its own error."""
+    shapes = [(8, 2, 128, [3000, 7], [1, 1], None), (32, 1, 128, [500], [40], "tree"), (4, 4, 64, [0, 900], [9, 3], None)]
+    trees = [Tree(BF16, BF16, *s[:3], 16, *s[3:], seed=56) for s in shapes]
+    want = [(t.run(pkg).o.clone(), t.lse.clone()) for t in trees]
+    dev = [[x.cuda() for x in (t.q, t.k, t.v, t.kc, t.vc, t.table)] + [ints(t.held), ints(t.starts)] for t in trees]
+    masks = [None if t.mask is None else t.mask.cuda() for t in trees]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            t = trees[i]
+            refused, why = ({"k_descale": 2.0}, "descales apply") if i == 1 else ({"scale": math.nan}, "scale must be finite")
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    o, lse = torch.full_like(want[i][0], 7), torch.full_like(want[i][1], 7)
+                    args = {"scale": t.scale, "mask": masks[i], "max_new": t.max_new, "output": o, "lse": lse}
+                    pkg.fused_tree(*dev[i], **args)
+                    with pytest.raises(pkg.AttentionError, match=why):
+                        pkg.fused_tree(*dev[i], **{**args, **refused})
+                    torch.cuda.current_stream().synchronize()
+                    if not (torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1])):
+                        wrong.append(i)
+        except BaseException as e:  # noqa: BLE001
+            wrong.append((i, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    pkg.check_status(0)
+    assert not wrong
